@@ -338,6 +338,96 @@ int zilla_lm_cache_reset(int net);
 /* KVCache::$length: the number of cached positions (>= 0), or a negative status. */
 int zilla_lm_cache_length(int net);
 
+/* ---- generation for a batch: rotary positions, a paged K/V cache, attention over
+ *      a shared prefix, drafted tokens (no reference counterpart: the reference
+ *      generates one sequence at a time with learned positions and one contiguous
+ *      cache, src/Generators/Sampler.php:35-100,
+ *      src/Attention/MultiHeadAttention.php:99-137) ----
+ *
+ * Element types: 0 fp32, 1 bf16, 2 fp16; a buffer of n 16-bit elements takes
+ * (n + 1) / 2 registry floats.  Integers (positions, lengths, page numbers,
+ * tokens) are int32 in a buffer, as argmax is.  Every buffer has to be large
+ * enough for the sizes given and on the current device (-1 and -2 otherwise).
+ * The calls only enqueue kernels (no allocation, no synchronisation), so they
+ * can be captured into a CUDA graph; what the host cannot see (a page number, a
+ * length, a drafted token out of range) is skipped by the kernel, which records
+ * it for zilla_check_device. */
+
+/* The table of rotary frequencies, rot_dim + 2 floats: rot_dim / 2 doubles (turns
+ * a position, pair i's base^(-2i/rot_dim) / 2 pi) and one double (the magnitude of
+ * the rotated part).  scaling: 0 none; 1 linear, frequencies / factor; 2 base *
+ * factor^(rot_dim / (rot_dim - 2)); 3 by parts: pairs that turn more than `fast`
+ * times in `original` positions keep their frequency, those below `slow` turns
+ * are divided by factor, linear between, and the magnitude is 0.1 ln factor + 1.
+ * rot_dim even, 2 to 256. */
+int rope_table_dev(int table_id, int rot_dim, float base, int scaling, float factor, int original, float slow,
+                   float fast);
+/* Rotates the first rot_dim elements of every head of x [rows][heads][head_dim]
+ * into y and copies the rest; row t at position pos[t] (any int32).  x_off, x_ld
+ * (and y_off, y_ld): the first head's offset in a row and the row stride, in
+ * elements, so the queries of a packed projection are rotated where they lie.
+ * interleaved 0: pairs (i, i + rot_dim / 2), 1: pairs (2i, 2i + 1).  inverse 1
+ * turns back with the same magnitude: the gradient of x from that of y.  x and
+ * y may be the same rows of one buffer.  head_dim 2 to 256. */
+int rope_dev(int x_id, int x_off, int x_ld, int y_id, int y_off, int y_ld, int pos_id, int table_id, int type,
+             int rows, int heads, int head_dim, int rot_dim, int interleaved, int inverse);
+
+/* A paged K/V cache: K and V [pages][kv_heads][page][head_dim], zeroed; page 16,
+ * 32, 64 or 128 tokens, head_dim 32, 64 or 128, type 1 or 2.  Returns an id > 0,
+ * or a negative status.  zilla_kv_k_id / zilla_kv_v_id: the registry handles
+ * (owned by the cache; do not free). */
+int zilla_kv_create(int pages, int page, int kv_heads, int head_dim, int type);
+int zilla_kv_destroy(int kv);
+int zilla_kv_k_id(int kv);
+int zilla_kv_v_id(int kv);
+
+/* The batch of the next two calls: new rows are packed, sequence b has rows
+ * start[b] .. start[b + 1] - 1 (none is allowed); len[b] tokens of its own are in
+ * the cache, the new ones included; its i-th own token lies in page
+ * pages[b * max_pages + i / page].  Every sequence stands behind the same
+ * prefix_len tokens (0: none), which lie in the pages of prefix_pages.  Rows
+ * behind the last sequence (start[batch] .. rows - 1) are left as they are.
+ *
+ * Appends the new rows' K and V, K rotated at position prefix_len + i, and writes
+ * the rotated Q to qout [rows][q_heads][head_dim] of the cache's type.  x_type: 0
+ * or the cache's type; *_off and *_ld: as rope_dev's, of each input (one packed
+ * projection, or three buffers).  q_heads 0: no Q.  rot_dim 0: no rotation (no
+ * table).  A prefix is filled by the same call: batch 1, its page list as pages,
+ * prefix_len 0. */
+int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id, int k_off, int k_ld, int v_id,
+                    int v_off, int v_ld, int qout_id, int start_id, int len_id, int pages_id, int batch, int rows,
+                    int q_heads, int max_pages, int prefix_len, int table_id, int rot_dim, int interleaved);
+/* out = softmax(scale q K^T) V for q and out [rows][q_heads][head_dim] of the
+ * cache's type, q_heads a multiple of kv_heads (each kv head serves q_heads /
+ * kv_heads query heads).  New row j of a sequence with n new rows sees the prefix
+ * and its own keys 0 .. len - n + j; a row that sees none (no prefix, len < n)
+ * becomes zero.  The prefix's K and V are read once for all sequences.  max_new
+ * and max_len bound every sequence's new rows and length (a sequence beyond them
+ * is recorded and its rows are left as they are).  Whatever lies in pages behind
+ * a sequence's length does not matter; V of the tokens within it has to be
+ * finite.  A page number outside the cache counts as keys and values of zero.
+ * work: zilla_kv_attend_work floats (0: work_id is not looked at) that no other
+ * call in flight uses. */
+int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int pages_id, int prefix_pages_id, int batch,
+                    int rows, int q_heads, int max_pages, int prefix_len, int max_new, int max_len, float scale,
+                    int work_id);
+long zilla_kv_attend_work(int kv, int batch, int rows, int q_heads, int prefix_len, int max_new, int max_len);
+
+/* Drafted tokens against the target's probabilities, from given random numbers
+ * (speculative sampling).  Sequence b's rows start[b] .. start[b + 1] - 1 are its k
+ * drafts and one row behind them (k = rows - 1; no row: nothing but accepted[b] = 0).
+ * With row i's target probabilities p_i (fp32, row stride p_ld >= vocab), drafter's
+ * q_i, draft d_i and number u_i in [0, 1): drafts are accepted in order while u_i
+ * q_i(d_i) < p_i(d_i).  Behind the a accepted ones a token is drawn, at a failure
+ * from max(p_a - q_a, 0) (from p_a where that is zero throughout), else from p_k:
+ * the lowest t whose sum of weights up to t is above u_k times the whole sum.
+ * tokens [rows]: the accepted drafts, the drawn token, then -1; accepted[b] = a.
+ * Sums are fp64.  q_id 0: drafts made with certainty (q is one at the draft).
+ * NaN and negative weights count as zero; u_k >= 1 takes the last token with a
+ * weight; no weight at all gives token 0.  A draft outside the vocabulary fails. */
+int draft_verify_dev(int p_id, int p_ld, int q_id, int q_ld, int draft_id, int u_id, int start_id, int tokens_id,
+                     int accepted_id, int batch, int rows, int vocab);
+
 /* ---- data-parallel runner (one process per GPU, NVLink) ----
  * zilla_dp_unique_id writes a 128-byte NCCL unique id (rank 0 creates it,
  * the host distributes it, e.g. through a file or a store).

@@ -1,0 +1,521 @@
+"""Rotary positions, the paged K/V cache, attention over a shared prefix and draft verification against plain 64-bit
+implementations, at the sizes and masks where they can go wrong."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import genref as R
+from zillaphp_b200 import native
+from zillaphp_b200.backend import B200Backend
+from zillaphp_b200.kv import PagedKv
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def bufs():
+    b = R.Buffers(B200Backend())
+    yield b
+    b.be.sync()
+    assert native.load().zilla_check_device() == 0, native.last_error()
+    b.close()
+
+
+def starts(new):
+    return [0] + list(np.cumsum(new).tolist())
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+# ---------------------------------------------------------------------------------------- rotary positions
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,heads,dim,rot,interleaved,scaling,inverse,off,ld,far", [
+    (1, 1, 2, 2, 0, 0, 0, 0, 0, 10),                  # the smallest
+    (1, 4, 32, 32, 0, 0, 0, 0, 0, 128),
+    (5, 3, 128, 64, 1, 3, 0, 8, 512, 1 << 20),        # part of the head, by parts, packed rows
+    (9, 2, 80, 26, 0, 1, 1, 3, 175, 1000),            # odd halves and offsets: one element at a time
+    (9, 2, 80, 28, 1, 1, 1, 2, 180, 1000),            # two at a time
+    (33, 5, 96, 88, 1, 2, 1, 4, 600, (1 << 31) - 1),  # four at a time, the farthest positions
+    (700, 40, 128, 128, 0, 0, 0, 0, 0, 131072),       # several rows a block
+    (17, 2, 256, 256, 1, 0, 1, 0, 0, 5),
+    (2500, 7, 64, 56, 0, 3, 0, 0, 0, 4096),
+])
+def test_rope(bufs, dtype, rows, heads, dim, rot, interleaved, scaling, inverse, off, ld, far):
+    g = torch.Generator().manual_seed(rows + rot)
+    wide = heads * dim
+    ld = ld or wide
+    x = torch.randn((rows, ld), generator=g).to(R.DT[dtype])
+    pos = torch.randint(-min(far, 100), far, (rows,), generator=g, dtype=torch.int64).to(torch.int32)
+    pos[0] = far if far < 2 ** 31 else far - 1
+    args = (10000.0, scaling, 8.0, 4096, 1.0, 32.0)
+    table = bufs.new(rot + 2)
+    bufs.be.ropeTableDev(table, rot, *args)
+    before = torch.randn((rows, wide + 8), generator=g).to(R.DT[dtype])
+    ix, iy, ip = bufs.put(x), bufs.put(before), bufs.put(pos)
+    bufs.be.ropeDev(ix, off, ld, iy, 4 if ld == wide else 0, wide + 8, ip, table, R.CODE[dtype], rows, heads, dim, rot, interleaved, inverse)
+    y = bufs.get(iy, before.shape, R.DT[dtype])
+    y_off = 4 if ld == wide else 0
+    ref, size = R.rotate(x[:, off:off + wide].reshape(rows, heads, dim), pos, rot, interleaved, R.rates(rot, *args), -1.0 if inverse else 1.0)
+    got = y[:, y_off:y_off + wide].reshape(rows, heads, dim).double()
+    tol = size * (R.ROTATION + R.far(pos)) + (R.half_step(ref, R.DT[dtype]) if dtype != "fp32" else 0)
+    assert ((got - ref).abs() <= tol).all(), float(((got - ref).abs() - tol).max())
+    assert torch.equal(got[..., rot:], ref[..., rot:])                       # copied bit for bit
+    keep = torch.ones(wide + 8, dtype=torch.bool)
+    keep[y_off:y_off + wide] = False
+    assert torch.equal(y[:, keep], before[:, keep])                         # nothing else is written
+
+
+def test_rope_in_place_in_a_packed_row(bufs):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((37, 6 * 64), generator=g)
+    pos = torch.arange(37, dtype=torch.int32)
+    table = bufs.new(66)
+    bufs.be.ropeTableDev(table, 64)
+    ix, ip = bufs.put(x), bufs.put(pos)
+    bufs.be.ropeDev(ix, 128, 384, ix, 128, 384, ip, table, 0, 37, 2, 64, 64)
+    y = bufs.get(ix, x.shape, torch.float32)
+    ref, size = R.rotate(x[:, 128:256].reshape(37, 2, 64), pos, 64, 0, R.rates(64))
+    assert ((y[:, 128:256].reshape(37, 2, 64).double() - ref).abs() <= size * R.ROTATION).all()
+    assert torch.equal(y[:, :128], x[:, :128]) and torch.equal(y[:, 256:], x[:, 256:])
+
+
+def test_rope_gradient_against_differences(bufs):
+    """The inverse turn is the gradient: central differences of f(x) = sum(w y(x)), linear in x, so that the step adds
+    only rounding (fp32 y: 2^-24 of about 4 each, over 16 elements and a step of 0.5)."""
+    g = torch.Generator().manual_seed(4)
+    rows, dim, rot = 2, 8, 6
+    x, w, pos = torch.randn((rows, 1, dim), generator=g), torch.randn((rows, 1, dim), generator=g), i32([3, 70000])
+    table = bufs.new(rot + 2)
+    bufs.be.ropeTableDev(table, rot, 10000.0, 3, 4.0, 64)
+    ip, iy = bufs.put(pos), bufs.new(x.numel())
+
+    def turn(t, inverse):
+        bufs.be.ropeDev(bufs.put(t), 0, dim, iy, 0, dim, ip, table, 0, rows, 1, dim, rot, 1, inverse)
+        return bufs.get(iy, t.shape, torch.float32).double()
+
+    grad = turn(w, 1)
+    for r in range(rows):
+        for i in range(dim):
+            e = torch.zeros_like(x)
+            e[r, 0, i] = 0.5
+            d = ((turn(x + e, 0) - turn(x - e, 0)) * w.double()).sum()
+            assert abs(float(d) - float(grad[r, 0, i])) < 16 * 4 * 2.0 ** -23 / 0.5
+
+
+# ---------------------------------------------------------------------------------------- the cache
+def batch_of(new, length, prefix, page, seed, max_pages=0, spare=3):
+    """start, pages, prefix pages and the number of pages, in no order."""
+    g = torch.Generator().manual_seed(seed)
+    most = max(max_pages, max(1, -(-max(list(length) + [1]) // page)))
+    first = max(1, -(-prefix // page))
+    order = torch.randperm(first + most * len(new) + spare, generator=g).to(torch.int32)
+    return starts(new), order[first:first + most * len(new)].reshape(len(new), most), order[:first], order.numel(), most
+
+
+@pytest.mark.parametrize("src,dtype", [("fp32", "bf16"), ("bf16", "bf16"), ("fp32", "fp16"), ("fp16", "fp16")])
+@pytest.mark.parametrize("new,length,hq,hk,dim,rot,interleaved,page,prefix,packed,pad", [
+    ([1], [1], 4, 4, 32, 32, 0, 16, 0, False, 0),
+    ([1, 0, 3], [17, 0, 16], 6, 2, 64, 24, 1, 16, 5, True, 2),        # a sequence without rows, rows behind the last
+    ([5, 2], [5, 130], 7, 1, 128, 128, 0, 128, 999999, False, 1),
+    ([40, 1, 300], [40, 64, 301], 8, 8, 128, 96, 1, 64, 70, True, 0),  # prompts, pages crossed
+    ([3], [70], 0, 2, 64, 64, 0, 32, 0, False, 0),                    # no queries
+    ([2, 2], [9, 3], 2, 1, 32, 0, 0, 16, 0, True, 0),                 # no rotation
+    ([2] * 300, [33] * 300, 2, 1, 32, 30, 0, 32, 3, False, 4),        # more sequences than threads
+])
+def test_append(bufs, src, dtype, new, length, hq, hk, dim, rot, interleaved, page, prefix, packed, pad):
+    start, pages, _, count, most = batch_of(new, length, 0, page, 5)
+    rows = start[-1] + pad
+    g = torch.Generator().manual_seed(6)
+    wide = (hq + 2 * hk) * dim
+    ld = wide + 24
+    x = torch.randn((max(rows, 1), ld), generator=g).to(R.DT[src])
+    q, k, v = x[:, 8:8 + hq * dim], x[:, 8 + hq * dim:8 + (hq + hk) * dim], x[:, 8 + (hq + hk) * dim:8 + wide]
+    kv = PagedKv(count, page, hk, dim, dtype)
+    shape = (count, hk, page, dim)
+    kc, vc = (torch.randn(shape, generator=g).to(R.DT[dtype]) for _ in range(2))
+    bufs.write(kv.k_id, kc)
+    bufs.write(kv.v_id, vc)
+    out = torch.randn((rows, max(hq, 1), dim), generator=g).to(R.DT[dtype])
+    table = 0
+    if rot:
+        table = bufs.new(rot + 2)
+        bufs.be.ropeTableDev(table, rot)
+    io = bufs.put(out)
+    if packed:
+        i = bufs.put(x)
+        inputs = (i, 8, ld, i, 8 + hq * dim, ld, i, 8 + (hq + hk) * dim, ld)
+    else:
+        inputs = (bufs.put(q) if hq else 0, 0, hq * dim, bufs.put(k), 0, hk * dim, bufs.put(v), 0, hk * dim)
+    kv.append(R.CODE[src], *inputs, io if hq else 0, bufs.put(i32(start)), bufs.put(i32(length)), bufs.put(pages), len(new), rows, hq,
+              most, prefix, table, rot, interleaved)
+    at = torch.tensor([length[b] - new[b] + j for b in range(len(new)) for j in range(new[b])], dtype=torch.long)
+    own = torch.tensor([b for b in range(len(new)) for _ in range(new[b])], dtype=torch.long)
+    n, T = start[-1], R.DT[dtype]
+    plan, pos = R.rates(rot) if rot else None, at + prefix
+    got = bufs.get(io, out.shape, T)
+    if hq:
+        ref, size = R.rotate(q[:n].reshape(n, hq, dim), pos, rot, interleaved, plan or ([], 1.0))
+        tol = size * (R.ROTATION + R.far(pos)) + R.half_step(ref, T)
+        assert ((got[:n].double() - ref).abs() <= tol).all()
+        assert torch.equal(got[n:], out[n:])
+    page_of, slot = pages[own, at // page].long(), at % page
+    ref, size = R.rotate(k[:n].reshape(n, hk, dim), pos, rot, interleaved, plan or ([], 1.0))
+    got_k, got_v = bufs.get(kv.k_id, shape, T), bufs.get(kv.v_id, shape, T)
+    tol = size * (R.ROTATION + R.far(pos)) + R.half_step(ref, T)
+    assert ((got_k[page_of, :, slot].double() - ref).abs() <= tol).all()
+    vc[page_of, :, slot] = v[:n].reshape(n, hk, dim).to(T)
+    assert torch.equal(got_v, vc)                                    # values rounded once, nothing else written
+    got_k[page_of, :, slot] = kc[page_of, :, slot]
+    assert torch.equal(got_k, kc)
+    kv.close()
+
+
+# ---------------------------------------------------------------------------------------- attention
+def run_attend(bufs, dtype, new, length, hq, hk, dim, page, prefix, pad=0, max_new=0, max_len=0, scale=None, max_pages=0, seed=7,
+               junk=True, sharp=1.5):
+    T = R.DT[dtype]
+    start, pages, front, count, most = batch_of(new, length, prefix, page, seed, max_pages)
+    rows = start[-1] + pad
+    g = torch.Generator().manual_seed(seed)
+    shape = (count, hk, page, dim)
+    k, v = (torch.randn(shape, generator=g).to(T) for _ in range(2))
+    kj, vj = k.clone(), v.clone()
+    if junk:   # every slot that no sequence holds: NaN, infinities
+        held = torch.zeros((count, page), dtype=torch.bool)
+        for i in range(prefix):
+            held[front[i // page], i % page] = True
+        for b, n in enumerate(length):
+            for i in range(n):
+                held[pages[b, i // page], i % page] = True
+        bad = torch.tensor([float("nan"), float("inf"), float("-inf")]).to(T)
+        m = ~held[:, None, :, None].expand(shape)
+        kj[m] = bad[torch.arange(int(m.sum())) % 3]
+        vj[m] = bad[torch.arange(int(m.sum())) % 3]
+    q = (torch.randn((rows, hq, dim), generator=g) * sharp).to(T)
+    out = torch.randn((rows, hq, dim), generator=g).to(T)
+    kv = PagedKv(count, page, hk, dim, dtype)
+    bufs.write(kv.k_id, kj)
+    bufs.write(kv.v_id, vj)
+    max_new, max_len = max_new or max(max(new), 1), max_len or max(length)
+    scale = 1 / math.sqrt(dim) if scale is None else scale
+    work = kv.attend_work(len(new), rows, hq, prefix, max_new, max_len)
+    io = bufs.put(out)
+    iw = bufs.new(work) if work else 0
+    if work:   # whatever the workspace holds does not matter
+        bufs.be.bufferUpload(iw, np.full(work, np.nan, np.float32))
+    kv.attend(bufs.put(q), io, bufs.put(i32(start)), bufs.put(i32(length)), bufs.put(pages), bufs.put(front), len(new), rows, hq, most,
+              prefix, max_new, max_len, scale, iw)
+    got = bufs.get(io, out.shape, T)
+    ref = R.attend(q, k, v, start, length, pages.tolist(), front.tolist(), prefix, scale, page)
+    n = start[-1]
+    tol = R.attend_tolerance(ref, dim, T)
+    assert torch.isfinite(got[:n]).all()
+    err = (got[:n].double() - ref[0][:n]).abs()
+    assert (err <= tol[:n]).all(), float((err / tol[:n]).max())
+    assert torch.equal(got[n:], out[n:])
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("new,length,hq,hk,page,prefix,pad", [
+    ([1], [1], 1, 1, 16, 0, 0),                              # one key: the smallest
+    ([1], [1], 1, 1, 16, 1, 0),
+    ([1, 0, 2], [1, 0, 64], 3, 1, 16, 15, 2),                # a sequence without rows, an odd group
+    ([1, 1, 1], [65, 63, 17], 4, 4, 64, 64, 0),              # a key past a stage, MHA
+    ([5, 1, 3], [200, 129, 3], 8, 2, 128, 130, 1),           # drafts, pages that end inside a stage
+    ([2, 4], [513, 40], 7, 1, 32, 0, 0),                     # no prefix, joined slots
+    ([6] * 5, [6, 70, 33, 100, 64], 16, 2, 32, 257, 3),      # more rows than one tile of 32
+    ([30, 1], [90, 20], 8, 2, 16, 40, 0),                    # a prompt in the middle: several row tiles
+    ([1, 2], [0, 1], 4, 2, 16, 33, 0),                       # rows in front of the first own key: the prefix alone
+])
+def test_attend(bufs, dtype, dim, new, length, hq, hk, page, prefix, pad):
+    run_attend(bufs, dtype, new, length, hq, hk, dim, page, prefix, pad)
+
+
+def test_attend_rows_without_keys(bufs):
+    run_attend(bufs, "bf16", [2, 1, 3], [0, 5, 1], 4, 2, 64, 16, 0, 1)       # joined or direct: zeros
+    run_attend(bufs, "bf16", [1, 2], [0, 0], 4, 2, 64, 16, 0, max_len=16)
+    run_attend(bufs, "fp16", [3, 1], [1, 400], 4, 2, 64, 16, 0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attend_loose_bounds(bufs, dtype):
+    """max_new and max_len far above what is there."""
+    run_attend(bufs, dtype, [1, 3], [20, 300], 8, 2, 128, 16, 100, 1, max_new=9, max_len=1000, max_pages=80)
+
+
+def test_attend_scales(bufs):
+    run_attend(bufs, "bf16", [1, 2], [100, 70], 4, 2, 64, 16, 90, scale=-0.3)
+    run_attend(bufs, "bf16", [1, 2], [100, 70], 4, 2, 64, 16, 90, scale=0.0)
+    run_attend(bufs, "bf16", [1, 2], [100, 70], 4, 2, 64, 16, 90, scale=0.4, sharp=8.0)   # one key takes nearly all
+
+
+@pytest.mark.parametrize("dtype,dim,hq,hk,prefix,new", [
+    ("bf16", 128, 32, 8, 1000, [1] * 33), ("fp16", 64, 32, 4, 777, [3, 1, 5, 2] * 4), ("bf16", 32, 4, 4, 300, [1] * 130),
+    ("bf16", 128, 5, 1, 129, [2] * 60), ("fp16", 128, 16, 2, 2049, [4] * 9)])
+def test_attend_many_rows_behind_one_prefix(bufs, dtype, dim, hq, hk, prefix, new):
+    length = [n + (7 * i) % 90 for i, n in enumerate(new)]
+    run_attend(bufs, dtype, new, length, hq, hk, dim, 64, prefix, 2)
+
+
+def test_attend_bad_numbers_are_recorded():
+    """A page number outside the cache counts as keys and values of zero; a length beyond the call's leaves its rows alone."""
+    b = R.Buffers(B200Backend())
+    kv = PagedKv(4, 16, 1, 32, "bf16")
+    ones = torch.ones((4, 1, 16, 32), dtype=torch.bfloat16)
+    b.write(kv.k_id, ones)
+    b.write(kv.v_id, ones)
+    q, out = torch.ones((2, 1, 32)).to(torch.bfloat16), torch.full((2, 1, 32), 7.0).to(torch.bfloat16)
+    io = b.put(out)
+    for page in (4, -1, 2 ** 31 - 1, -2 ** 31):
+        kv.attend(b.put(q), io, b.put(i32([0, 1, 2])), b.put(i32([16, 999])), b.put(i32([[page], [0]])), 0, 2, 2, 1, 1, 0, 1, 16, 1.0,
+                  b.new(max(1, kv.attend_work(2, 2, 1, 0, 1, 16))))
+        got = b.get(io, out.shape, torch.bfloat16)
+        assert (got[0] == 0).all() and (got[1] == 7).all()
+        assert native.load().zilla_check_device() == -3
+        assert native.load().zilla_check_device() == 0
+    table, x = b.new(34), b.put(torch.ones((2, 32)))
+    b.be.ropeTableDev(table, 32)
+    kv.append(0, x, 0, 32, x, 0, 32, x, 0, 32, io, b.put(i32([0, 1, 2])), b.put(i32([1, 17])), b.put(i32([[9], [0]])), 2, 2, 1, 1, 0, table, 32)
+    assert native.load().zilla_check_device() == -3            # a bad page, and a token behind the table's end
+    assert torch.equal(b.get(kv.k_id, ones.shape, torch.bfloat16), ones) and torch.equal(b.get(io, out.shape, torch.bfloat16), got)
+    kv.close()
+    b.close()
+
+
+# ---------------------------------------------------------------------------------------- verification
+def rows_of(new, vocab, ld, seed, near=0.7):
+    g = np.random.default_rng(seed)
+    rows = sum(new)
+    z = g.standard_normal((rows, vocab)) * 2
+    e = np.exp(z)
+    p = np.zeros((rows, ld), np.float32)
+    q = np.zeros((rows, ld), np.float32)
+    p[:, :vocab] = e / e.sum(1, keepdims=True)
+    e = np.exp(z + g.standard_normal((rows, vocab)) * near)
+    q[:, :vocab] = e / e.sum(1, keepdims=True)
+    draft = np.array([g.choice(vocab, p=(r[:vocab].astype(np.float64) / r[:vocab].astype(np.float64).sum())) for r in q], np.int32).reshape(-1)
+    return p, q, draft, g.random(rows, np.float32)
+
+
+def run_verify(bufs, p, q, draft, u, new, vocab, pad=0):
+    start, rows, ld = starts(new), p.shape[0], p.shape[1]
+    before = np.full(rows + pad, -7, np.int32)
+    it, ia = bufs.put(torch.from_numpy(before)), bufs.put(torch.full((len(new),), -7, dtype=torch.int32))
+    zeros = np.zeros((pad, ld), np.float32)
+    bufs.be.draftVerifyDev(bufs.put(torch.from_numpy(np.concatenate([p, zeros]))), ld,
+                           0 if q is None else bufs.put(torch.from_numpy(np.concatenate([q, zeros]))), ld,
+                           bufs.put(torch.from_numpy(np.concatenate([draft, np.zeros(pad, np.int32)]))),
+                           bufs.put(torch.from_numpy(np.concatenate([u, np.zeros(pad, np.float32)]))), bufs.put(i32(start)), it, ia,
+                           len(new), rows + pad, vocab)
+    tokens, accepted = R.verify(p, q, draft, u, start, vocab)
+    got = bufs.get(it, (rows + pad,), torch.int32).tolist()
+    assert bufs.get(ia, (len(new),), torch.int32).tolist() == accepted
+    assert got[:rows] == [tokens[i] for i in range(rows)] and got[rows:] == [-7] * pad
+    return accepted
+
+
+@pytest.mark.parametrize("vocab,ld", [(1, 1), (2, 4), (65, 65), (129, 132), (4096, 4096), (5001, 5003), (33333, 33336), (131072, 131072)])
+@pytest.mark.parametrize("certain", [False, True])
+def test_verify(bufs, vocab, ld, certain):
+    for seed, new in enumerate(([1], [5, 1, 0, 9, 2], [3] * 40 if vocab < 6000 else [4] * 6)):
+        p, q, draft, u = rows_of(new, vocab, ld, seed)
+        run_verify(bufs, p, None if certain else q, draft, u, new, vocab, 2)
+
+
+def test_verify_borders(bufs):
+    """Equal probabilities, numbers of 0 and next to 1, every draft taken, none taken, over 32 drafts."""
+    new = [40, 40, 3]
+    p, q, draft, u = rows_of(new, 300, 300, 11, near=0.0)
+    q[:] = p
+    u[:] = np.float32(1 - 2.0 ** -24)
+    assert run_verify(bufs, p, q, draft, u, new, 300) == [39, 39, 2]        # u q < p for every u < 1
+    u[35] = 0.0
+    p[35, draft[35]] = 0.0                                                   # 0 < 0 fails: the 36th draft
+    q[45] *= np.float32(1.5)                                                 # the 6th of the second
+    u[39] = u[79] = u[82] = 0.0
+    assert run_verify(bufs, p, q, draft, u, new, 300) == [35, 5, 2]
+    u[39] = u[79] = u[82] = np.float32(1.0)                                  # above every border: the last with a weight
+    run_verify(bufs, p, q, draft, u, new, 300)
+
+
+def test_verify_degenerate_rows(bufs):
+    """No residual, zeros throughout, NaN, negative and infinite values."""
+    new = [2, 2, 2, 2, 1]
+    p, q, draft, u = rows_of(new, 50, 50, 12)
+    q[0] = np.float32(2.0) * p[0] + 1                # fails, nothing left: drawn from p
+    p[2] = 0.0                                       # fails, and no weight at all: token 0
+    p[4, 10:20] = np.nan
+    p[4, draft[4]] = 0.0
+    p[6, draft[6]] = 0.0
+    p[6, 5] = -1.0
+    u[0] = u[4] = u[6] = 0.9
+    run_verify(bufs, p, q, draft, u, new, 50)
+
+
+def test_verify_bad_drafts_are_recorded():
+    b = R.Buffers(B200Backend())
+    new = [3, 2]
+    p, q, draft, u = rows_of(new, 40, 40, 13)
+    u[:] = 0.0
+    draft[1], draft[3] = 40, -2 ** 31
+    assert run_verify(b, p, q, draft, u, new, 40) == [1, 0]
+    assert native.load().zilla_check_device() == -3
+    it, ia = b.put(torch.full((5,), -7, dtype=torch.int32)), b.put(i32([9, 9]))
+    b.be.draftVerifyDev(b.put(torch.from_numpy(p)), 40, 0, 0, b.put(torch.from_numpy(draft)), b.put(torch.from_numpy(u)), b.put(i32([0, 6, 5])),
+                        it, ia, 2, 5, 40)                                      # rows that do not fit
+    assert b.get(ia, (2,), torch.int32).tolist() == [0, 0] and b.get(it, (5,), torch.int32).tolist() == [-7] * 5
+    assert native.load().zilla_check_device() == -3
+    b.close()
+
+
+# ---------------------------------------------------------------------------------------- together
+class Loop:
+    """Generation steps as a program runs them: a shared prompt, then rounds of drafted tokens for every sequence."""
+
+    def __init__(self, bufs, dtype="bf16", hq=8, hk=2, dim=64, page=16, prefix=37, size=5, most=4, seed=21):
+        self.b, self.dtype, self.hq, self.hk, self.dim, self.page, self.prefix, self.size, self.most = bufs, dtype, hq, hk, dim, page, prefix, size, most
+        self.rows, self.max_len, self.vocab = size * most, 96, 65
+        self.g = torch.Generator().manual_seed(seed)
+        self.wide = (hq + 2 * hk) * dim
+        own_pages, front = self.max_len // page, -(-prefix // page)
+        order = torch.randperm(own_pages * size + front, generator=self.g).to(torch.int32)
+        self.front, self.pages = order[:front], order[front:].reshape(size, own_pages)
+        self.kv = PagedKv(order.numel(), page, hk, dim, dtype)
+        self.table = bufs.new(dim + 2)
+        bufs.be.ropeTableDev(self.table, dim)
+        self.ids = {n: bufs.new(w) for n, w in (("x", self.rows * self.wide), ("q", self.rows * hq * dim), ("out", self.rows * hq * dim),
+                                                 ("start", size + 1), ("len", size), ("draft", self.rows), ("u", self.rows), ("p", self.rows * 65),
+                                                 ("tokens", self.rows), ("accepted", size), ("logits", self.rows * 65), ("head", hq * dim * 65))}
+        self.ids["pages"], self.ids["front"] = bufs.put(self.pages), bufs.put(self.front)
+        self.ids["work"] = bufs.new(max(1, self.kv.attend_work(size, self.rows, hq, prefix, most, self.max_len)))
+        self.k_ref = torch.zeros((order.numel(), hk, page, dim), dtype=R.DT[dtype])
+        self.v_ref = self.k_ref.clone()
+        x = torch.randn((prefix, self.wide), generator=self.g)
+        i = bufs.put(x)
+        self.kv.append(0, 0, 0, 0, i, hq * dim, self.wide, i, (hq + hk) * dim, self.wide, 0, bufs.put(i32([0, prefix])), bufs.put(i32([prefix])),
+                       self.ids["front"], 1, prefix, 0, front, 0, self.table, dim)
+        self.store(x, torch.arange(prefix), self.front[torch.arange(prefix) // page].long(), torch.arange(prefix) % page)
+        self.length = [0] * size
+
+    def store(self, x, pos, page_of, slot):
+        n, a, c = x.shape[0], self.hq * self.dim, (self.hq + self.hk) * self.dim
+        k, _ = R.rotate(x[:, a:c].reshape(n, self.hk, self.dim), pos, self.dim, 0, R.rates(self.dim))
+        self.k_ref[page_of, :, slot] = k.to(self.k_ref.dtype)
+        self.v_ref[page_of, :, slot] = x[:, c:].reshape(n, self.hk, self.dim).to(self.k_ref.dtype)
+
+    def new_step(self, new):
+        """Uploads one step's inputs."""
+        self.new, self.start = new, starts(new)
+        self.length = [a + n for a, n in zip(self.length, new)]
+        self.x = torch.randn((self.rows, self.wide), generator=self.g)
+        self.draft = torch.randint(0, self.vocab, (self.rows,), generator=self.g, dtype=torch.int32)
+        self.u = torch.rand((self.rows,), generator=self.g)
+        logits = torch.randn((self.rows, self.vocab), generator=self.g)
+        for name, t in (("x", self.x), ("start", i32(self.start)), ("len", i32(self.length)), ("draft", self.draft), ("u", self.u), ("logits", logits)):
+            self.b.write(self.ids[name], t)
+
+    def calls(self):
+        d, i, hq, hk = self.dim, self.ids, self.hq, self.hk
+        self.kv.append(0, i["x"], 0, self.wide, i["x"], hq * d, self.wide, i["x"], (hq + hk) * d, self.wide, i["q"], i["start"], i["len"], i["pages"],
+                       self.size, self.rows, hq, self.pages.shape[1], self.prefix, self.table, d)
+        self.kv.attend(i["q"], i["out"], i["start"], i["len"], i["pages"], i["front"], self.size, self.rows, hq, self.pages.shape[1], self.prefix,
+                       self.most, self.max_len, 1 / math.sqrt(d), i["work"])
+        self.b.be.softmaxRowsFwdDev(i["logits"], i["p"], self.rows, self.vocab)
+        self.b.be.draftVerifyDev(i["p"], self.vocab, 0, 0, i["draft"], i["u"], i["start"], i["tokens"], i["accepted"], self.size, self.rows, self.vocab)
+
+    def check(self):
+        n, T = self.start[-1], R.DT[self.dtype]
+        own = torch.tensor([b for b in range(self.size) for _ in range(self.new[b])], dtype=torch.long)
+        at = torch.tensor([self.length[b] - self.new[b] + j for b in range(self.size) for j in range(self.new[b])], dtype=torch.long)
+        self.store(self.x[:n], at + self.prefix, self.pages[own, at // self.page].long(), at % self.page)
+        # attention on the cache and queries as the device holds them: their own roundings are the append's test
+        q = self.b.get(self.ids["q"], (self.rows, self.hq, self.dim), T)
+        k, v = (self.b.get(i, self.k_ref.shape, T) for i in (self.kv.k_id, self.kv.v_id))
+        assert torch.equal(v, self.v_ref)
+        # a key's rounding may fall to the other side of a border that the rotation's error reaches: one step
+        assert ((k.double() - self.k_ref.double()).abs() <= 2.01 * R.half_step(torch.maximum(k.abs(), self.k_ref.abs()), T)).all()
+        ref = R.attend(q, k, v, self.start, self.length, self.pages.tolist(), self.front.tolist(), self.prefix, 1 / math.sqrt(self.dim), self.page)
+        got = self.b.get(self.ids["out"], (self.rows, self.hq, self.dim), T)
+        tol = R.attend_tolerance(ref, self.dim, T)
+        assert ((got[:n].double() - ref[0][:n]).abs() <= tol[:n]).all()
+        p = self.b.get(self.ids["p"], (self.rows, self.vocab), torch.float32).numpy()
+        tokens, accepted = R.verify(p, None, self.draft.numpy(), self.u.numpy(), self.start, self.vocab)
+        got = self.b.get(self.ids["tokens"], (self.rows,), torch.int32).tolist()
+        assert [got[i] for i in range(n)] == [tokens[i] for i in range(n)]
+        assert self.b.get(self.ids["accepted"], (self.size,), torch.int32).tolist() == accepted
+        # the refused drafts leave the cache: the next step writes over them
+        self.length = [m - n + a + 1 if n else m for m, n, a in zip(self.length, self.new, accepted)]
+
+
+STEPS = ([1, 4, 2, 0, 3], [4, 4, 4, 4, 4], [0, 1, 0, 2, 0], [3, 2, 1, 4, 1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_generation_steps(bufs, dtype):
+    loop = Loop(bufs, dtype)
+    for new in STEPS:
+        loop.new_step(list(new))
+        loop.calls()
+        loop.check()
+    loop.kv.close()
+
+
+def test_generation_steps_captured_on_another_stream(bufs):
+    """The calls captured once on a stream of the program's own and replayed for each step."""
+    lib = native.load()
+    loop = Loop(bufs)
+    loop.new_step(list(STEPS[0]))
+    loop.calls()
+    loop.check()
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    bufs.be.sync()
+    try:
+        with torch.cuda.graph(graph, stream=s):
+            lib.zilla_set_stream(C.c_void_p(s.cuda_stream))
+            loop.calls()
+        for new in STEPS[1:]:
+            loop.new_step(list(new))
+            with torch.cuda.stream(s):
+                graph.replay()
+            loop.check()
+    finally:
+        lib.zilla_set_stream(None)
+    loop.kv.close()
+
+
+def test_two_captured_calls_with_their_own_workspaces(bufs):
+    """Two graphs of the same attention, each with its workspace, in flight on two streams: bit for bit the eager results."""
+    lib = native.load()
+    loops = [Loop(bufs, seed=s, prefix=300, page=16) for s in (1, 2)]
+    want, graphs, streams = [], [], [torch.cuda.Stream() for _ in loops]
+    for loop in loops:
+        loop.new_step([4, 1, 4, 2, 4])
+        loop.calls()
+        want.append(bufs.get(loop.ids["out"], (loop.rows, loop.hq, loop.dim), torch.bfloat16))
+    bufs.be.sync()
+    try:
+        for loop, s in zip(loops, streams):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                lib.zilla_set_stream(C.c_void_p(s.cuda_stream))
+                loop.calls()
+            graphs.append(g)
+        for _ in range(20):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+    finally:
+        lib.zilla_set_stream(None)
+    for loop, w in zip(loops, want):
+        n = loop.start[-1]
+        assert torch.equal(bufs.get(loop.ids["out"], w.shape, torch.bfloat16)[:n], w[:n])
+        loop.kv.close()

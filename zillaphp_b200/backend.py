@@ -188,6 +188,20 @@ class B200Backend:
     def causalSoftmaxDev(self, xId, N, M, maskValue=-1e9):  # noqa: N802,N803
         self._check(self.ffi.causal_softmax_dev(xId, N, M, maskValue), "causal_softmax_dev")
 
+    # ------------------------------------------------------------ generation
+    def ropeTableDev(self, tableId, rotDim, base=10000.0, scaling=0, factor=1.0, original=1, slow=1.0, fast=32.0):  # noqa: N802,N803,E501
+        self._check(self.ffi.rope_table_dev(tableId, rotDim, base, scaling, factor, original, slow, fast),
+                    "rope_table_dev")
+
+    def ropeDev(self, xId, xOff, xLd, yId, yOff, yLd, posId, tableId, type, rows, heads, headDim, rotDim,  # noqa: A002,N802,N803,E501
+                interleaved=0, inverse=0):
+        self._check(self.ffi.rope_dev(xId, xOff, xLd, yId, yOff, yLd, posId, tableId, type, rows, heads, headDim, rotDim,
+                                      interleaved, inverse), "rope_dev")
+
+    def draftVerifyDev(self, pId, pLd, qId, qLd, draftId, uId, startId, tokensId, acceptedId, batch, rows, vocab):  # noqa: N802,N803,E501
+        self._check(self.ffi.draft_verify_dev(pId, pLd, qId, qLd, draftId, uId, startId, tokensId, acceptedId, batch, rows,
+                                              vocab), "draft_verify_dev")
+
     # ------------------------------------------------------------ host-pointer helpers
     def matmul(self, a: np.ndarray, b: np.ndarray) -> np.ndarray:
         a = np.ascontiguousarray(a, np.float32)

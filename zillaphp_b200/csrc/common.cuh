@@ -5,6 +5,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <initializer_list>
+
 #include "../../include/zilla_b200.h"
 
 namespace zb {
@@ -30,6 +32,17 @@ void count_launch(unsigned n = 1);
 float *ptr(int id);
 // Capacity in floats of a registry handle (0 if invalid).
 size_t capacity(int id);
+
+// One buffer argument of an entry point: its handle, the floats that the call
+// reads or writes in it, and its name in the error text.
+struct BufferNeed {
+    int id;
+    size_t floats;
+    const char *what;
+};
+// kBadHandle for an unknown handle or a buffer that is too small, kBadArg for a
+// buffer on another device than the current one, else kOk.
+int check_buffers(const char *name, std::initializer_list<BufferNeed> needs);
 
 // Programmatic dependent launch.  A kernel started by launch_pdl may begin
 // while the previous kernel on the stream is still running: it calls

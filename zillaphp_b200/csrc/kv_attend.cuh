@@ -1,0 +1,104 @@
+// kv_attend.cuh -- attention of a batch's new tokens over a prefix that all
+// sequences share and over each sequence's own cached keys: the parameters
+// and the parts that its kernels share.
+//
+// For row j of sequence b (n new rows, len own cached tokens) and one query head:
+//   o = sum_i softmax_i(scale q.k_i) v_i over the prefix's keys and the own keys i < len - n + j + 1.
+// The keys are cut into slots (prefix_splits of the prefix, own_splits of the own keys); a slot's kernel
+// leaves the row's maximum m (in units of log2), its sum l = sum 2^(s - m) and o = sum 2^(s - m) v in
+// fp32, and the join takes sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c in slot order.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace zb {
+namespace kv {
+
+struct AttendParams {
+    CUtensorMap k_map, v_map;
+    const void *q;
+    void *out;
+    float *part_o;      // [slots][rows * q_heads][head_dim]
+    float2 *part_ml;    // [slots][rows * q_heads]
+    KvBatch batch;
+    const int *prefix_pages;
+    int q_heads, kv_heads, group, page_log2, pages, box_rows;
+    int max_new, max_len;
+    int prefix_splits, prefix_chunk, own_splits, own_chunk;   // slots, and keys of a slot
+    int prefix_tiles, own_tiles;                              // row tiles of this launch
+    int prefix_items;                                         // blocks [0, prefix_items) take the prefix
+    int direct;         // one slot in all: its kernel writes out itself
+    float scale_log2;
+    int *err;
+};
+
+// Keys that row j of a sequence sees of its own: clamped to 0 .. len.
+__device__ __forceinline__ int own_limit(int len, int n, int j) { return max(0, len - n + j + 1); }
+
+// A sequence's new rows and length; one that does not fit the call's sizes is recorded and has no rows.
+__device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int &first, int &n, int &len) {
+    first = p.batch.start[b];
+    n = p.batch.start[b + 1] - first;
+    len = p.batch.len[b];
+    if (first < 0 || n < 0 || n > p.max_new || (long long)first + n > p.batch.rows || len < 0 || len > p.max_len) {
+        atomicCAS(p.err, 0, kErrKvLength);
+        n = 0;
+        len = 0;
+    }
+}
+
+// The TMA row coordinate of the box at `key` of a page list: the cache's end (a box of zeros) behind
+// `end` and for a page number outside the cache, which is recorded.
+__device__ __forceinline__ int box_row(const AttendParams &p, const int *pages, int kv_head, int key, int end) {
+    const int none = p.pages * p.kv_heads << p.page_log2;
+    if (key >= end) return none;
+    const int id = pages[key >> p.page_log2];
+    if (id < 0 || id >= p.pages) {
+        atomicCAS(p.err, 0, kErrKvPage);
+        return none;
+    }
+    return ((id * p.kv_heads + kv_head) << p.page_log2) + (key & ((1 << p.page_log2) - 1));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// D += A B, one warp's 16 x 8 tile with K = 16, fp32 accumulation.
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Byte offset of the 16-byte chunk of a key row in a tile that TMA wrote: 128-byte rows whose chunks are
+// XORed with the row's low three bits (64-byte rows, head_dim 32: with bits 1 and 2), one such block of
+// 64 rows for each 64 elements of the head.
+template <int D>
+__device__ __forceinline__ uint32_t tile_chunk(int row, int chunk, int rows) {
+    if constexpr (D == 32) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    else return (chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+}  // namespace kv
+}  // namespace zb

@@ -1,0 +1,52 @@
+// kv_cache.cuh -- the paged K/V cache object (zilla_kv_create) and the batch
+// description that its append and its attention share.
+//
+// K and V are [pages][kv_heads][page][head_dim], bf16 or fp16: one head's keys of one page are
+// contiguous, so a TMA box fetches them and a page's rows fill whole 128-byte lines.
+#pragma once
+
+#include "half_types.cuh"
+#include "tc_common.cuh"
+
+namespace zb {
+
+struct KvCache {
+    int pages = 0, page = 0, page_log2 = 0, kv_heads = 0, head_dim = 0, type = kBf16;
+    int k_id = 0, v_id = 0;
+    void *k = nullptr, *v = nullptr;
+    CUtensorMap k_map, v_map;   // [pages * kv_heads * page][head_dim], box {min(head_dim, 64), box_rows}
+    int box_rows = 0;           // rows of one TMA box: a page, 64 at most
+};
+
+// The cache of an id; nullptr when unknown, or when one of its buffers was freed.
+const KvCache *kv_get(int id);
+
+// Error codes of the device error word.
+enum KvErr : int {
+    kErrKvLength = 0x4b560001,   // a sequence's rows or length do not fit the call's sizes
+    kErrKvPage = 0x4b560002,     // a page number outside the cache, or a token behind the page table's end
+    kErrDraft = 0x4b560003,      // a drafted token outside the vocabulary, or rows that do not fit
+};
+
+// The batch's packed rows: sequence b has the new rows start[b] .. start[b + 1] - 1 and len[b] tokens
+// of its own in the cache, those included.
+struct KvBatch {
+    const int *start, *len, *pages;   // pages: [batch][max_pages]
+    int batch, rows, max_pages, prefix_len;
+};
+
+// The sequences of the block's rows row0 .. row0 + n - 1 into owner[] (shared memory; -1 behind the
+// last sequence).  Every thread looks at batch / threads sequences, so there is no chain of dependent
+// loads as in a search.  Ends with the block synchronised.
+__device__ __forceinline__ void kv_owners(int *owner, const int *__restrict__ start, int batch, int row0, int n,
+                                          int tid, int threads) {
+    for (int i = tid; i < n; i += threads) owner[i] = -1;
+    __syncthreads();
+    for (int b = tid; b < batch; b += threads) {
+        const int lo = max(start[b], row0), hi = min(start[b + 1], row0 + n);
+        for (int t = lo; t < hi; ++t) owner[t - row0] = b;
+    }
+    __syncthreads();
+}
+
+}  // namespace zb

@@ -18,6 +18,7 @@ struct Slot {
     float *p;
     size_t n;
     int used;
+    int device;   // the device the memory is on
 };
 Slot g_slots[kSlots];
 cudaStream_t g_own_stream = nullptr;
@@ -30,18 +31,27 @@ int g_sms = 0;
 }  // namespace
 
 namespace {
-int *g_err_word = nullptr;
+constexpr int kMaxDevices = 64;
+int *g_err_word[kMaxDevices] = {};   // each device's own: a kernel never writes to a peer's
 }
 
 int *device_error_word() {
-    if (!g_err_word) {
-        if (cudaMalloc((void **)&g_err_word, sizeof(int)) != cudaSuccess) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    int *&w = g_err_word[dev];
+    if (!w) {
+        if (cudaMalloc((void **)&w, sizeof(int)) != cudaSuccess) {
             cudaGetLastError();
+            w = nullptr;
             return nullptr;
         }
-        cudaMemsetAsync(g_err_word, 0, sizeof(int), stream());
+        cudaMemsetAsync(w, 0, sizeof(int), stream());
+        cudaStreamSynchronize(stream());   // cleared before a kernel of any other stream can write to it
     }
-    return g_err_word;
+    return w;
 }
 
 int fail(int status, const char *fmt, ...) {
@@ -75,6 +85,20 @@ float *ptr(int id) {
 size_t capacity(int id) {
     if (id <= 0 || id >= kSlots || !g_slots[id].used) return 0;
     return g_slots[id].n;
+}
+
+int check_buffers(const char *name, std::initializer_list<BufferNeed> needs) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return check_cuda(name);
+    for (const BufferNeed &b : needs) {
+        if (!ptr(b.id)) return fail(kBadHandle, "%s: invalid handle %d (%s)", name, b.id, b.what);
+        if (g_slots[b.id].n < b.floats)
+            return fail(kBadHandle, "%s: %s needs %zu floats, its buffer has %zu", name, b.what, b.floats, g_slots[b.id].n);
+        if (g_slots[b.id].device != dev)
+            return fail(kBadArg, "%s: %s is on device %d, the current device is %d", name, b.what,
+                        g_slots[b.id].device, dev);
+    }
+    return kOk;
 }
 
 int sm_count() {
@@ -121,7 +145,10 @@ int zilla_buffer_alloc(unsigned long n_floats) {
             cudaGetLastError();
             return fail(kBadHandle, "zilla_buffer_alloc: cudaMalloc of %zu bytes failed", bytes);
         }
-        g_slots[i] = {p, (size_t)n_floats, 1};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        g_slots[i] = {p, (size_t)n_floats, 1, dev};
+        device_error_word();   // exists before any op on a buffer runs, so an op's first call may be captured
         return i;
     }
     return fail(kBadHandle, "zilla_buffer_alloc: no free slots");
@@ -131,7 +158,7 @@ void zilla_buffer_free(int id) {
     if (id <= 0 || id >= kSlots || !g_slots[id].used) return;
     cudaStreamSynchronize(stream());
     cudaFree(g_slots[id].p);
-    g_slots[id] = {nullptr, 0, 0};
+    g_slots[id] = {nullptr, 0, 0, 0};
 }
 
 int zilla_buffer_upload(int id, const float *host, unsigned long n_floats) {

@@ -102,6 +102,16 @@ SIGNATURES: dict[str, tuple] = {
     "zilla_lm_cache_reset": (I, [I]),
     "zilla_lm_set_precision": (I, [I, I]),
     "zilla_lm_cache_length": (I, [I]),
+    "rope_table_dev": (I, [I, I, F, I, F, I, F, F]),
+    "rope_dev": (I, [I] * 15),
+    "zilla_kv_create": (I, [I] * 5),
+    "zilla_kv_destroy": (I, [I]),
+    "zilla_kv_k_id": (I, [I]),
+    "zilla_kv_v_id": (I, [I]),
+    "zilla_kv_append": (I, [I] * 23),
+    "zilla_kv_attend": (I, [I] * 14 + [F, I]),
+    "zilla_kv_attend_work": (C.c_long, [I] * 7),
+    "draft_verify_dev": (I, [I] * 12),
     "zilla_dp_unique_id": (I, [C.c_char_p]),
     "zilla_dp_attach": (I, [I, I, I, C.c_char_p]),
     "zilla_dp_detach": (I, [I]),
