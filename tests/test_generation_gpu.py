@@ -258,10 +258,16 @@ def test_attend_scales(bufs):
 
 @pytest.mark.parametrize("dtype,dim,hq,hk,prefix,new", [
     ("bf16", 128, 32, 8, 1000, [1] * 33), ("fp16", 64, 32, 4, 777, [3, 1, 5, 2] * 4), ("bf16", 32, 4, 4, 300, [1] * 130),
-    ("bf16", 128, 5, 1, 129, [2] * 60), ("fp16", 128, 16, 2, 2049, [4] * 9)])
+    ("bf16", 128, 5, 1, 129, [2] * 60), ("fp16", 128, 16, 2, 2049, [4] * 9),
+    ("bf16", 128, 32, 8, 2500, [4] * 70), ("fp16", 32, 66, 1, 128, [1]), ("bf16", 64, 130, 2, 1, [3, 1]), ("fp16", 128, 28, 4, 640, [6] * 40)])
 def test_attend_many_rows_behind_one_prefix(bufs, dtype, dim, hq, hk, prefix, new):
     length = [n + (7 * i) % 90 for i, n in enumerate(new)]
     run_attend(bufs, dtype, new, length, hq, hk, dim, 64, prefix, 2)
+
+
+def test_attend_many_rows_scales(bufs):
+    for scale, sharp in ((-0.2, 1.5), (0.0, 1.5), (0.4, 8.0)):
+        run_attend(bufs, "bf16", [2] * 20, [20] * 20, 8, 1, 64, 16, 700, scale=scale, sharp=sharp)
 
 
 def test_attend_bad_numbers_are_recorded():

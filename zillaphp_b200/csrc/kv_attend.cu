@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "kv_attend.cuh"
+#include "kv_attend_tc.cuh"
 
 namespace zb {
 namespace kv {
@@ -307,6 +308,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
 
 // ---------------------------------------------------------------- plan
 struct Plan {
+    bool tc;                // the prefix on tcgen05
     int own_wm, prefix_wm;
     int own_tiles, prefix_tiles, own_chunk, own_splits, prefix_chunk, prefix_splits;
     bool direct;
@@ -315,25 +317,43 @@ struct Plan {
 
 int row_warps(long long rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
+// Rows that share the prefix's keys from which it goes to tcgen05.
+constexpr int kTcRows = 64;
+
 // Row tiles of 16, 32 or 64 rows by the rows that share the keys, and slots of whole 64-key stages such
 // that all blocks together are about `kWaves` rounds of two blocks an SM: fewer would leave SMs idle, more would
-// add parts to write and join.
+// add parts to write and join.  The tcgen05 kernel runs one block an SM: its slots minimise rounds x (tiles
+// of a block + kTcFixed tiles for its start and end).
 Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_len, int max_new, int max_len) {
-    constexpr int kWaves = 2;
+    constexpr int kWaves = 2, kTcFixed = 3;
     Plan p;
     const int group = q_heads / c.kv_heads;
     const long long own_rows = (long long)max_new * group, prefix_rows = (long long)rows * group;
+    p.tc = prefix_rows > kTcRows && prefix_len > 0;
     p.own_wm = row_warps(own_rows);
     p.prefix_wm = row_warps(prefix_rows);
     p.own_tiles = (int)((own_rows + 16 * p.own_wm - 1) / (16 * p.own_wm));
-    p.prefix_tiles = (int)((prefix_rows + 16 * p.prefix_wm - 1) / (16 * p.prefix_wm));
+    const int tile_rows = p.tc ? 2 * kTcTile : 16 * p.prefix_wm;
+    p.prefix_tiles = (int)((prefix_rows + tile_rows - 1) / tile_rows);
     const long long own_steps = (max_len + kTile - 1) / kTile, prefix_steps = (prefix_len + kTile - 1) / kTile;
-    const long long total = c.kv_heads * (own_steps * batch * p.own_tiles + prefix_steps * p.prefix_tiles);
+    const long long total = c.kv_heads * (own_steps * batch * p.own_tiles + (p.tc ? 0 : prefix_steps * p.prefix_tiles));
     const long long per = std::max<long long>(1, total / (2LL * kWaves * sm_count()));
     p.own_chunk = (int)std::min(per, std::max(1LL, own_steps)) * kTile;
     p.own_splits = (int)((max_len + p.own_chunk - 1) / p.own_chunk);
     p.prefix_chunk = (int)std::min(per, std::max(1LL, prefix_steps)) * kTile;
-    p.prefix_splits = (prefix_len + p.prefix_chunk - 1) / p.prefix_chunk;
+    if (p.tc) {
+        const long long tiles = (prefix_len + kTcTile - 1) / kTcTile;
+        long long best = 0;
+        for (long long s = 1; s <= std::min(tiles, 64LL); ++s) {
+            const long long chunk = (tiles + s - 1) / s, slots = (tiles + chunk - 1) / chunk;
+            const long long rounds = (slots * p.prefix_tiles * c.kv_heads + sm_count() - 1) / sm_count(), cost = rounds * (chunk + kTcFixed);
+            if (s == 1 || cost < best) {
+                best = cost;
+                p.prefix_chunk = (int)chunk * kTcTile;
+            }
+        }
+    }
+    p.prefix_splits = (int)(((long long)prefix_len + p.prefix_chunk - 1) / p.prefix_chunk);
     if (p.own_splits + p.prefix_splits == 0) p.own_splits = 1;   // no keys at all: the rows are still written
     p.direct = p.own_splits == 1 && p.prefix_splits == 0;
     p.units = (size_t)rows * q_heads;
@@ -341,16 +361,22 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
     return p;
 }
 
+// Shared memory above 48 KB is asked for once a device.
+template <typename K>
+int allow_smem(K kernel, int bytes, bool (&set)[64], const char *name) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && set[dev]) return kOk;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (int rc = check_cuda(name)) return rc;
+    if (dev >= 0 && dev < 64) set[dev] = true;
+    return kOk;
+}
+
 template <typename T, int D, int WM>
 int launch_split(const AttendParams &p, long long blocks, const char *name) {
     static bool set[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !set[dev]) {
-        cudaFuncSetAttribute(attend_split_kernel<T, D, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem<D>());
-        if (int rc = check_cuda(name)) return rc;
-        if (dev >= 0 && dev < 64) set[dev] = true;
-    }
+    if (int rc = allow_smem(attend_split_kernel<T, D, WM>, split_smem<D>(), set, name)) return rc;
     if (blocks > 0x7fffffffLL) return fail(kBadArg, "%s: %lld blocks are too many", name, blocks);
     launch_pdl(attend_split_kernel<T, D, WM>, dim3((unsigned)blocks), dim3(kSplitThreads), split_smem<D>(), p);
     ZB_LAUNCH_CHECK(name);
@@ -369,7 +395,13 @@ int run(AttendParams p, const Plan &plan, const char *name) {
     const long long own = (long long)p.batch.batch * p.own_splits * p.own_tiles * p.kv_heads;
     const long long prefix = (long long)p.prefix_splits * p.prefix_tiles * p.kv_heads;
     if (prefix > 0x7fffffffLL) return fail(kBadArg, "%s: %lld blocks are too many", name, prefix);
-    if (plan.own_wm == plan.prefix_wm) {
+    if (plan.tc) {
+        static bool set[64] = {};
+        if (int rc = allow_smem(attend_tc_kernel<T, D>, tc_smem<D>(), set, name)) return rc;
+        launch_pdl(attend_tc_kernel<T, D>, dim3((unsigned)prefix), dim3(kTcThreads), tc_smem<D>(), p);
+        ZB_LAUNCH_CHECK(name);
+        if (int rc = run_split<T, D>(p, plan.own_wm, own, name)) return rc;
+    } else if (plan.own_wm == plan.prefix_wm) {
         p.prefix_items = (int)prefix;
         if (int rc = run_split<T, D>(p, plan.own_wm, prefix + own, name)) return rc;
     } else {

@@ -1,0 +1,345 @@
+// kv_attend_tc.cuh -- the shared prefix's part of zilla_kv_attend on tcgen05, for batches whose rows
+// (tokens x query heads of a kv head) fill 128-row tiles.
+//
+// One block takes two 128-row tiles ("streams"), one kv head and one slot of the prefix's keys; both
+// streams use each K and V tile of 128 keys, so a tile crosses L2 once for 256 rows.  Per tile and stream:
+//   S = Q K^T          M = 128 rows, N = 128 keys, K = head_dim, fp32 in TMEM
+//   P = 2^(S - ref)    one thread a row; P (16 bits) replaces S in TMEM, two keys a column
+//   O += P V           A = P from TMEM, B = V [key][d] (N-major), N = head_dim, fp32 in TMEM
+// ref is the row's maximum as of its last change: it follows the true maximum only when that has passed it
+// by 2^8 (then O and l are rescaled), so that O rarely has to travel through registers; weights stay
+// below 2^8 and l and O carry the same factor, so the quotient does not change.
+// Warps 0-3 and 4-7 are the streams' softmax, warp 8 loads (TMA through the page list), warp 9 issues the
+// MMAs: while one stream's softmax runs, the other's MMAs do.
+//
+// Order of the MMAs of a stream: P V of tile j, then Q K^T of tile j + 1 over the same TMEM columns; one
+// thread issues both and the tensor pipe takes them in order.  S's barrier of tile j + 1 is a commit behind
+// P V of tile j, so a softmax that sees it may also rescale O.
+#pragma once
+
+#include "kv_attend.cuh"
+
+namespace zb {
+namespace kv {
+
+using namespace tc;
+
+constexpr int kTcTile = 128;      // rows of a stream, keys of a tile
+constexpr int kTcThreads = 320;
+
+template <int D>
+constexpr int tc_stages() { return D == 128 ? 5 : 8; }
+template <int D>
+constexpr int tc_smem() { return (2 + tc_stages<D>()) * kTcTile * D * 2 + 1024 + 256; }
+
+template <typename T>
+constexpr uint32_t attend_idesc(int n, bool b_mn) {
+    return __is_same(T, __half) ? (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24)
+                                : idesc_bf16(128, n, false, b_mn);
+}
+
+// D += A B with A in TMEM (16-bit elements, two a column).
+__device__ __forceinline__ void mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+// 32 lanes x 32 columns, without the wait.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+// Waits for the thread's TMEM loads; the registers pass through, so nothing that reads them moves ahead.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_constant__ AttendParams p) {
+    constexpr int ST = tc_stages<D>(), kTileBytes = kTcTile * D * 2, kHalves = D == 128 ? 2 : 1, kRowBytes = D < 64 ? D * 2 : 128;
+    constexpr int kHalfBytes = kTcTile * 128;                       // one 64-column block of a tile (D >= 64)
+    constexpr Swizzle kSw = D == 32 ? kSw64 : kSw128;
+    constexpr uint32_t kAtom = D == 32 ? 512 : 1024;                // eight rows
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t *base = smem_raw + (((raw + 1023u) & ~1023u) - raw);    // Q of both streams, then the ring
+    uint8_t *ring = base + 2 * kTileBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + ST * kTileBytes);
+    uint64_t *full = bars, *empty = bars + ST, *q_full = bars + 2 * ST, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 2, *drain = o_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    int item = blockIdx.x;
+    const int pair = item % p.prefix_tiles;
+    item /= p.prefix_tiles;
+    const int head = item % p.kv_heads, slot = item / p.kv_heads;
+    const int rows = p.batch.rows * p.group, row0 = pair * 2 * kTcTile;
+    const int streams = rows - row0 > kTcTile ? 2 : 1;
+    const int begin = slot * p.prefix_chunk, end = min(begin + p.prefix_chunk, p.batch.prefix_len);
+    const int tiles = (end - begin + kTcTile - 1) / kTcTile;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        mbar_init(q_full, streams * kTcTile);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(s_full + s, 1);
+            mbar_init(p_full + s, kTcTile);
+            mbar_init(o_full + s, 1);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    griddep_launch();
+    griddep_wait();
+
+    if (warp == 8) {
+        // ---- loads: K and V tiles alternate through the ring
+        const int boxes = kTcTile / p.box_rows, all = boxes * kHalves;   // 2 .. 16
+        const int r0 = lane % boxes * p.box_rows, half = lane / boxes;
+        bool ok = true;
+        int i = 0;
+        for (; i < 2 * tiles; ++i) {
+            const int st = i % ST;
+            const int at = lane < all ? box_row(p, p.prefix_pages, head, begin + (i >> 1) * kTcTile + r0, end) : 0;
+            ok = i < ST || mbar_wait(empty + st, (i / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(full + st, kTileBytes);
+            __syncwarp();
+            if (lane < all)
+                tma_load_2d(ring + st * kTileBytes + half * kHalfBytes + r0 * kRowBytes, i & 1 ? &p.v_map : &p.k_map, full + st, half * 64, at);
+        }
+        if (!ok && lane == 0)   // the copies in flight end before the block's shared memory goes
+            for (int x = max(0, i - ST); x < i; ++x)
+                if (!mbar_wait_drain(full + x % ST, (x / ST) & 1)) atomicCAS(p.err, 0, kErrDrain);
+    } else if (warp == 9) {
+        // ---- MMAs
+        if (lane == 0) {
+            constexpr uint32_t kIdS = attend_idesc<T>(kTcTile, false), kIdO = attend_idesc<T>(D, true);
+            auto wait_tile = [&](int i) { return mbar_wait(full + i % ST, (i / ST) & 1, abort_flag, p.err, kErrFullWait); };
+            auto qk = [&](int s, int i) {
+                const uint32_t a = smem_u32(base) + s * kTileBytes, b = smem_u32(ring) + i % ST * kTileBytes;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = (k >> 2) * kHalfBytes + (k & 3) * 32;
+                    mma_bf16(tmem + s * 128, smem_desc(a + at, 16, kAtom, kSw), smem_desc(b + at, 16, kAtom, kSw), kIdS, k != 0);
+                }
+                mma_commit(s_full + s);
+            };
+            auto pv = [&](int s, int i, bool more) {
+                const uint32_t b = smem_u32(ring) + i % ST * kTileBytes;
+#pragma unroll
+                for (int k = 0; k < kTcTile / 16; ++k)
+                    mma_f16_ta(tmem + 256 + s * D, tmem + s * 128 + 8 * k, smem_desc(b + k * 2 * kAtom, kHalfBytes, kAtom, kSw), kIdO, more || k != 0);
+            };
+            bool ok = mbar_wait(q_full, 0, abort_flag, p.err, kErrFullWait) && wait_tile(0);
+            if (ok) {
+                tc_fence_after();
+                for (int s = 0; s < streams; ++s) qk(s, 0);
+                mma_commit(empty);
+            }
+            for (int j = 0; ok && j < tiles; ++j) {
+                ok = wait_tile(2 * j + 1);
+                for (int s = 0; ok && s < streams; ++s) {
+                    ok = mbar_wait(p_full + s, j & 1, abort_flag, p.err, kErrAccWait);
+                    if (!ok) break;
+                    tc_fence_after();
+                    pv(s, 2 * j + 1, j > 0);
+                    if (j + 1 == tiles) {
+                        mma_commit(o_full + s);
+                    } else {
+                        ok = s > 0 || wait_tile(2 * j + 2);
+                        if (!ok) break;
+                        tc_fence_after();
+                        qk(s, 2 * j + 2);
+                    }
+                }
+                if (!ok) break;
+                mma_commit(empty + (2 * j + 1) % ST);
+                if (j + 1 < tiles) mma_commit(empty + (2 * j + 2) % ST);
+            }
+            if (!ok) {   // MMAs in flight end before TMEM goes
+                mma_commit(drain);
+                if (!mbar_wait_drain(drain, 0)) atomicCAS(p.err, 0, kErrDrain);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 4 * streams) {
+        // ---- softmax: thread = row of the stream
+        const int s = warp >> 2, r = threadIdx.x & (kTcTile - 1), row = row0 + s * kTcTile + r;
+        const bool real = row < rows;
+        const int t = real ? row / p.group : 0, hq = head * p.group + (real ? row - t * p.group : 0);
+        const size_t unit = (size_t)t * p.q_heads + hq;
+        {
+            // with a negative scale the queries change their sign, so that the largest product has the largest score
+            const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + unit * D);
+            const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                uint4 x = real ? src[c] : make_uint4(0, 0, 0, 0);
+                x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                *reinterpret_cast<uint4 *>(base + s * kTileBytes + tile_chunk<D>(r, c, kTcTile)) = x;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_full);
+        }
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + s * 128, to = tmem + lanes + 256 + s * D;
+        const float sl = fmaxf(fabsf(p.scale_log2), 1e-30f);   // above zero: a masked -inf stays one
+        const uint64_t sl2 = pack_f32x2(sl, sl);
+        float ref = 0.0f, l = 0.0f;   // ref in units of log2
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            ok = mbar_wait(s_full + s, j & 1, abort_flag, p.err, kErrAccWait);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t v[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32_async(ts + 32 * c, v[c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld_wait(v[c]);
+            const int left = end - (begin + j * kTcTile);
+            if (left < kTcTile) {   // the last tile's missing keys; V behind them counts as zero, whatever its page holds
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (32 * c + i >= left) v[c][i] = 0xff800000u;
+                const int st = (2 * j + 1) % ST;
+                ok = mbar_wait(full + st, ((2 * j + 1) / ST) & 1, abort_flag, p.err, kErrFullWait);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                for (int x = r; x < (kTcTile - left) * (D / 8); x += kTcTile)
+                    *reinterpret_cast<uint4 *>(ring + st * kTileBytes + tile_chunk<D>(left + x / (D / 8), x % (D / 8), kTcTile)) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+            }
+            float top[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                top[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+                for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(v[c][i]));
+            }
+            float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
+            if (!(m > -INFINITY)) m = j ? ref : 0.0f;   // no key yet
+            if (j == 0) ref = m;
+            else if (__any_sync(0xffffffffu, m > ref + 8.0f)) {
+                const float f = m > ref ? ex2(ref - m) : 1.0f;
+                ref = fmaxf(ref, m);
+                l *= f;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32_async(to + 32 * c, o);
+                    tmem_ld_wait(o);
+                    uint32_t w[2][16];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) w[i >> 4][i & 15] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st16(to + 32 * c, w[0]);
+                    tmem_st16(to + 32 * c + 16, w[1]);
+                }
+            }
+            const uint64_t nref = pack_f32x2(-ref, -ref);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sl2, nref));
+                    const float a = ex2(x.x), b = ex2(x.y);
+                    sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(a, b));
+                    w[i] = pack2<T>(a, b);
+                }
+                tmem_st16(ts + 16 * c, w);
+            }
+            const float2 add = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+            l += add.x + add.y;
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(p_full + s);
+        }
+        if (ok) ok = mbar_wait(o_full + s, 0, abort_flag, p.err, kErrAccWait);
+        if (__all_sync(0xffffffffu, ok)) {
+            tc_fence_after();
+            const size_t at = (size_t)slot * p.batch.rows * p.q_heads + unit;
+            float4 *dst = reinterpret_cast<float4 *>(p.part_o + at * D);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32_async(to + 32 * c, o);
+                tmem_ld_wait(o);
+                if (real)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        dst[8 * c + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                                     __uint_as_float(o[4 * i + 3]));
+            }
+            if (real) p.part_ml[at] = make_float2(ref, l);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace kv
+}  // namespace zb
