@@ -57,39 +57,55 @@ __device__ __forceinline__ T from_f32(float v) {
     else return __float2bfloat16_rn(v);
 }
 
-// V elements of T at p as fp32; p is aligned to V elements (16 bytes at most are needed).
+// V elements of T as they lie in memory, loaded in accesses of 16 bytes at most (p aligned to V elements, 16
+// bytes suffice): kept like this while more loads are in flight, a 16-bit vector takes half of fp32's registers.
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T *p, float (&v)[V]) {
-    if constexpr (V == 1) {
-        v[0] = to_f32(*p);
-    } else if constexpr (sizeof(T) == 4) {
-        if constexpr (V == 2) {
-            const float2 a = *reinterpret_cast<const float2 *>(p);
-            v[0] = a.x; v[1] = a.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V / 4; ++i) {
-                const float4 a = reinterpret_cast<const float4 *>(p)[i];
-                v[4 * i] = a.x; v[4 * i + 1] = a.y; v[4 * i + 2] = a.z; v[4 * i + 3] = a.w;
-            }
-        }
+struct RawVec {
+    static constexpr int kWords = V * (int)sizeof(T) / 4;   // 0: one 16-bit element
+    uint32_t w[kWords > 0 ? kWords : 1];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ RawVec<T, V> load_raw(const T *p) {
+    RawVec<T, V> r;
+    constexpr int N = RawVec<T, V>::kWords;
+    if constexpr (N == 0) {
+        r.w[0] = *reinterpret_cast<const uint16_t *>(p);
+    } else if constexpr (N == 1) {
+        r.w[0] = *reinterpret_cast<const uint32_t *>(p);
+    } else if constexpr (N == 2) {
+        const uint2 a = *reinterpret_cast<const uint2 *>(p);
+        r.w[0] = a.x; r.w[1] = a.y;
     } else {
-        uint32_t w[V / 2];
-        if constexpr (V == 2) {
-            w[0] = *reinterpret_cast<const uint32_t *>(p);
-        } else if constexpr (V == 4) {
-            const uint2 a = *reinterpret_cast<const uint2 *>(p);
-            w[0] = a.x; w[1] = a.y;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4 *>(p);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 a = reinterpret_cast<const uint4 *>(p)[i];
+            r.w[4 * i] = a.x; r.w[4 * i + 1] = a.y; r.w[4 * i + 2] = a.z; r.w[4 * i + 3] = a.w;
         }
+    }
+    return r;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void widen(const RawVec<T, V> &r, float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = __uint_as_float(r.w[i]);
+    } else if constexpr (V == 1) {
+        v[0] = unpack2<T>(r.w[0]).x;
+    } else {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
-            const float2 f = unpack2<T>(w[i]);
+            const float2 f = unpack2<T>(r.w[i]);
             v[2 * i] = f.x; v[2 * i + 1] = f.y;
         }
     }
+}
+
+// V elements of T at p as fp32.
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T *p, float (&v)[V]) {
+    widen<T, V>(load_raw<T, V>(p), v);
 }
 
 template <typename T, int V>

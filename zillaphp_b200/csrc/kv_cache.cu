@@ -11,113 +11,89 @@ namespace {
 std::map<int, KvCache *> g_caches;
 int g_next_cache = 1;
 
-constexpr int kAppendThreads = 256;
-constexpr int kAppendTokens = 8;
-
 struct AppendParams {
     const void *q, *k, *v;
     void *q_out, *k_cache, *v_cache;
     long long q_ld, k_ld, v_ld;
     const double *table;   // nullptr: no rotation
     KvBatch batch;
-    int q_heads, kv_heads, page_log2, pages, tokens;
+    int q_heads, kv_heads, page_log2, pages;
     RopeShape shape;
-    FastDiv per_row, per_head;   // units of a row over all q, k and v heads; units of a head
+    RopeGrid grid;   // over the q, k and v heads together
     int *err;
 };
 
-// Bound by HBM for prompts (each element read and written once) and by latency for single tokens: one
-// block finds its rows' sequences, slots and angles together, then moves all heads.
-template <typename TI, typename TO, int V>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
-    __shared__ int owner[kAppendTokens], pos[kAppendTokens], page_of[kAppendTokens], slot[kAppendTokens];
-    __shared__ float2 cs[kAppendTokens * kRopeMaxDim / 2];
+// Bound by HBM for prompts (each element read and written once) and by latency for single tokens.  Where a
+// row comes from does not depend on its sequence, so a thread's first loads are under way while the block finds its
+// rows' sequences (a look at every start) and slots.
+template <typename TI, typename TO, int V, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) kv_append_kernel(const AppendParams p) {
+    __shared__ int owner[kRopeThreads];
     griddep_launch();
     griddep_wait();
-    const int tid = threadIdx.x, row0 = blockIdx.x * p.tokens, n = min(p.tokens, p.batch.rows - row0);
-    const int half_rot = p.shape.rot >> 1;
-    kv_owners(owner, p.batch.start, p.batch.batch, row0, n, tid, kAppendThreads);
-    if (tid < n) {
-        const int b = owner[tid];
-        int at_pos = 0, id = -1, s = 0;
-        if (b >= 0) {
-            const int first = p.batch.start[b], count = p.batch.start[b + 1] - first, held = p.batch.len[b];
-            const int i = held - count + (row0 + tid - first), at = i >> p.page_log2;
-            if (i < 0) {
-                atomicCAS(p.err, 0, kErrKvLength);
-            } else if (at >= p.batch.max_pages) {
-                atomicCAS(p.err, 0, kErrKvPage);
-            } else {
-                id = p.batch.pages[(size_t)b * p.batch.max_pages + at];
-                if (id < 0 || id >= p.pages) {
-                    atomicCAS(p.err, 0, kErrKvPage);
-                    id = -1;
-                }
-                at_pos = p.batch.prefix_len + i;
-                s = i & ((1 << p.page_log2) - 1);
-            }
+    const int u = threadIdx.x % p.shape.units, rest = threadIdx.x / p.shape.units, lane = rest % p.grid.lanes;
+    const int in_block = rest / p.grid.lanes, row0 = blockIdx.x * p.grid.rows, n = min(p.grid.rows, p.batch.rows - row0);
+    const bool works = in_block < n;
+    const size_t row = row0 + (works ? in_block : 0);
+    const int step = p.grid.lanes * p.grid.splits, D = p.shape.head_dim, heads = works ? p.q_heads + 2 * p.kv_heads : 0;
+    using Form = RopeForm<V, INTER>;
+    RopeLane<V, INTER> lane_of;
+    lane_of.place(u, p.shape);
+    RopeUnit<TI, V, Form::kTwo> unit[Form::kBatch];
+    const TI *q = static_cast<const TI *>(p.q) + row * p.q_ld, *k = static_cast<const TI *>(p.k) + row * p.k_ld - p.q_heads * D,
+             *v = static_cast<const TI *>(p.v) + row * p.v_ld - (p.q_heads + p.kv_heads) * D;
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < Form::kBatch; ++i) {
+            const int h = h0 + i * step;
+            if (h < heads) unit[i].load((h < p.q_heads ? q : h < p.q_heads + p.kv_heads ? k : v) + h * D, lane_of.at);
         }
-        page_of[tid] = id;   // -1: the row is left alone
-        slot[tid] = s;
-        pos[tid] = at_pos;
+    };
+    int h0 = blockIdx.y * p.grid.lanes + lane;
+    load(h0);
+    kv_owners(owner, p.batch.start, p.batch.batch, row0, n, threadIdx.x, blockDim.x);
+    const int b = works ? owner[in_block] : -1;
+    if (b < 0) return;
+    const int first = p.batch.start[b], own = p.batch.len[b] - (p.batch.start[b + 1] - first) + ((int)row - first), at = own >> p.page_log2;
+    if (own < 0 || at >= p.batch.max_pages) {
+        atomicCAS(p.err, 0, own < 0 ? kErrKvLength : kErrKvPage);
+        return;
     }
-    __syncthreads();
-    if (half_rot) {
-        rope_angles(cs, pos, n, half_rot, p.table, 1.0f, tid, kAppendThreads);
-        __syncthreads();
+    const int id = p.batch.pages[(size_t)b * p.batch.max_pages + at];
+    if (p.shape.rot) lane_of.angles(u, p.batch.prefix_len + own, p.shape, p.table, 1.0f);
+    if (id < 0 || id >= p.pages) {
+        atomicCAS(p.err, 0, kErrKvPage);
+        return;
     }
-    const int D = p.shape.head_dim;
-    const RopeShape turn = p.shape;
-    RopeShape copy = p.shape;   // the values: the same units, none turned; a pair unit then copies two vectors
-    const int total = n * (int)p.per_row.d;
-#pragma unroll 2
-    for (int idx = tid; idx < total; idx += kAppendThreads) {
-        const int t = p.per_row.div(idx), in_row = idx - t * (int)p.per_row.d;
-        int h = p.per_head.div(in_row);
-        const int u = in_row - h * (int)p.per_head.d;
-        const int id = page_of[t];
-        if (id < 0) continue;
-        const float2 *c = cs + t * half_rot;
-        if (h < p.q_heads) {
-            rope_unit<TI, TO, V>(static_cast<const TI *>(p.q) + (size_t)(row0 + t) * p.q_ld + h * D,
-                                 static_cast<TO *>(p.q_out) + ((size_t)(row0 + t) * p.q_heads + h) * D, c, u, turn);
-            continue;
+    TO *q_out = static_cast<TO *>(p.q_out) + row * p.q_heads * D;
+    const size_t slot = (((size_t)id * p.kv_heads) << p.page_log2) + (own & ((1 << p.page_log2) - 1));
+    while (h0 < heads) {
+#pragma unroll
+        for (int i = 0; i < Form::kBatch; ++i) {
+            int h = h0 + i * step;
+            if (h >= heads) continue;
+            TO *dst = q_out + h * D;
+            h -= p.q_heads;
+            const bool is_v = h >= p.kv_heads;   // values are copied
+            if (h >= 0) dst = static_cast<TO *>(is_v ? p.v_cache : p.k_cache) + (slot + ((size_t)(is_v ? h - p.kv_heads : h) << p.page_log2)) * D;
+            lane_of.finish(unit[i], dst, !is_v);
         }
-        h -= p.q_heads;
-        const bool is_k = h < p.kv_heads;
-        if (!is_k) h -= p.kv_heads;
-        const size_t to = ((((size_t)id * p.kv_heads + h) << p.page_log2) + slot[t]) * D;
-        if (is_k) {
-            rope_unit<TI, TO, V>(static_cast<const TI *>(p.k) + (size_t)(row0 + t) * p.k_ld + h * D,
-                                 static_cast<TO *>(p.k_cache) + to, c, u, turn);
-        } else {
-            const TI *src = static_cast<const TI *>(p.v) + (size_t)(row0 + t) * p.v_ld + h * D;
-            TO *dst = static_cast<TO *>(p.v_cache) + to;
-            float a[V];
-            if (u < copy.pair_units) {
-                const int a_at = copy.interleaved ? 2 * u * V : u * V;
-                const int b_at = copy.interleaved ? a_at + V : half_rot + u * V;
-                float b[V];
-                load_vec<TI, V>(src + a_at, a);
-                load_vec<TI, V>(src + b_at, b);
-                store_vec<TO, V>(dst + a_at, a);
-                store_vec<TO, V>(dst + b_at, b);
-            } else {
-                const int at = copy.rot + (u - copy.pair_units) * V;
-                load_vec<TI, V>(src + at, a);
-                store_vec<TO, V>(dst + at, a);
-            }
-        }
+        h0 += Form::kBatch * step;
+        load(h0);
     }
 }
 
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool INTER>
 void launch_append(const AppendParams &p, int vec) {
-    const dim3 grid((p.batch.rows + p.tokens - 1) / p.tokens), block(kAppendThreads);
-    if (vec == 8) launch_pdl(kv_append_kernel<TI, TO, 8>, grid, block, 0, p);
-    else if (vec == 4) launch_pdl(kv_append_kernel<TI, TO, 4>, grid, block, 0, p);
-    else if (vec == 2) launch_pdl(kv_append_kernel<TI, TO, 2>, grid, block, 0, p);
-    else launch_pdl(kv_append_kernel<TI, TO, 1>, grid, block, 0, p);
+    const dim3 grid((unsigned)((p.batch.rows + (long long)p.grid.rows - 1) / p.grid.rows), p.grid.splits), block(p.grid.threads);
+    if constexpr (sizeof(TI) == 2)
+        if (vec == 8) {
+            launch_pdl(kv_append_kernel<TI, TO, 8, INTER>, grid, block, 0, p);
+            return;
+        }
+    if (vec == 4) launch_pdl(kv_append_kernel<TI, TO, 4, INTER>, grid, block, 0, p);
+    else if (vec == 2) launch_pdl(kv_append_kernel<TI, TO, 2, INTER>, grid, block, 0, p);
+    else launch_pdl(kv_append_kernel<TI, TO, 1, INTER>, grid, block, 0, p);
 }
 
 }  // namespace
@@ -243,7 +219,7 @@ int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id,
     if (rot_dim)
         if (int rc = check_buffers(name, {{table_id, (size_t)rot_dim + 2, "table"}})) return rc;
     if (!rows || !batch) return kOk;
-    const int vec = rope_vector(D, rot_dim, {q_heads ? q_off : 0, q_heads ? q_ld : 0, k_off, k_ld, v_off, v_ld});
+    const int vec = rope_vector(x_type == kF32 ? 4 : 8, D, rot_dim, interleaved, {q_heads ? q_off : 0, q_heads ? q_ld : 0, k_off, k_ld, v_off, v_ld});
     const size_t es = elem_size(x_type);
     AppendParams p;
     p.q = q_heads ? reinterpret_cast<const char *>(ptr(q_id)) + q_off * es : nullptr;
@@ -265,19 +241,17 @@ int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id,
     p.shape = rope_shape(D, rot_dim, interleaved != 0, vec);
     p.err = device_error_word();
     if (!p.err) return fail(kBadHandle, "%s: no device error word", name);
-    const int per_row = (q_heads + 2 * c->kv_heads) * p.shape.units;
-    // as rope_dev: four units a thread where every SM still gets two blocks
-    int tokens = 1;
-    while (tokens < kAppendTokens && tokens * per_row < 4 * kAppendThreads && rows / (2 * tokens) >= 2 * sm_count()) tokens *= 2;
-    p.tokens = tokens;
-    p.per_row = FastDiv(per_row);
-    p.per_head = FastDiv(p.shape.units);
+    p.grid = rope_grid(rows, q_heads + 2 * c->kv_heads, p.shape.units);
+    auto launch = [&](auto in, auto out) {
+        if (interleaved) launch_append<decltype(in), decltype(out), true>(p, vec);
+        else launch_append<decltype(in), decltype(out), false>(p, vec);
+    };
     if (c->type == kBf16) {
-        if (x_type == kF32) launch_append<float, __nv_bfloat16>(p, vec);
-        else launch_append<__nv_bfloat16, __nv_bfloat16>(p, vec);
+        if (x_type == kF32) launch(float(), __nv_bfloat16());
+        else launch(__nv_bfloat16(), __nv_bfloat16());
     } else {
-        if (x_type == kF32) launch_append<float, __half>(p, vec);
-        else launch_append<__half, __half>(p, vec);
+        if (x_type == kF32) launch(float(), __half());
+        else launch(__half(), __half());
     }
     ZB_LAUNCH_CHECK(name);
     return kOk;

@@ -7,9 +7,6 @@
 namespace zb {
 namespace {
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeTokens = 8;   // rows of a block at most
-
 // One thread a pair.  Scaling:
 //   0  f_i = base^(-2i/rot) / 2 pi
 //   1  positions divided by factor (linear interpolation)
@@ -41,44 +38,56 @@ struct RopeParams {
     const int *pos;
     const double *table;
     long long x_ld, y_ld;
-    int rows, tokens;         // rows, and rows of a block
+    int rows, heads;
     RopeShape shape;
-    FastDiv per_row, per_head;   // units of a row, units of a head
+    RopeGrid grid;
     float sign;
 };
 
-// Bound by HBM: each element is read and written once.  A block's angles are worked out once into
-// shared memory for all heads of its rows.
-template <typename T, int V>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
-    __shared__ int pos[kRopeTokens];
-    __shared__ float2 cs[kRopeTokens * kRopeMaxDim / 2];
+// Bound by HBM: each element is read and written once, by whole warps along a head.
+template <typename T, int V, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_kernel(const RopeParams p) {
     griddep_launch();
     griddep_wait();
-    const int row0 = blockIdx.x * p.tokens, n = min(p.tokens, p.rows - row0), half_rot = p.shape.rot >> 1;
-    if (threadIdx.x < n) pos[threadIdx.x] = p.pos[row0 + threadIdx.x];
-    __syncthreads();
-    rope_angles(cs, pos, n, half_rot, p.table, p.sign, threadIdx.x, kRopeThreads);
-    __syncthreads();
-    const T *x = static_cast<const T *>(p.x) + (size_t)row0 * p.x_ld;
-    T *y = static_cast<T *>(p.y) + (size_t)row0 * p.y_ld;
-    const int total = n * (int)p.per_row.d;
-#pragma unroll 2
-    for (int k = threadIdx.x; k < total; k += kRopeThreads) {
-        const int t = p.per_row.div(k), in_row = k - t * (int)p.per_row.d;
-        const int h = p.per_head.div(in_row), u = in_row - h * (int)p.per_head.d;
-        const int at = h * p.shape.head_dim;
-        rope_unit<T, T, V>(x + t * p.x_ld + at, y + t * p.y_ld + at, cs + t * half_rot, u, p.shape);
+    const int u = threadIdx.x % p.shape.units, rest = threadIdx.x / p.shape.units, lane = rest % p.grid.lanes;
+    const long long row = (long long)blockIdx.x * p.grid.rows + rest / p.grid.lanes;
+    if (rest >= p.grid.rows * p.grid.lanes || row >= p.rows) return;
+    const int step = p.grid.lanes * p.grid.splits, D = p.shape.head_dim;
+    using Form = RopeForm<V, INTER>;
+    RopeLane<V, INTER> lane_of;
+    lane_of.place(u, p.shape);
+    const T *x = static_cast<const T *>(p.x) + row * p.x_ld;
+    T *y = static_cast<T *>(p.y) + row * p.y_ld;
+    const int pos = p.pos[row];
+    RopeUnit<T, V, Form::kTwo> unit[Form::kBatch];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < Form::kBatch; ++i)
+            if (h0 + i * step < p.heads) unit[i].load(x + (h0 + i * step) * D, lane_of.at);
+    };
+    int h0 = blockIdx.y * p.grid.lanes + lane;
+    load(h0);   // under way while the angles are worked out
+    lane_of.angles(u, pos, p.shape, p.table, p.sign);
+    while (h0 < p.heads) {
+#pragma unroll
+        for (int i = 0; i < Form::kBatch; ++i)
+            if (h0 + i * step < p.heads) lane_of.finish(unit[i], y + (h0 + i * step) * D, true);
+        h0 += Form::kBatch * step;
+        load(h0);
     }
 }
 
-template <typename T>
+template <typename T, bool INTER>
 void launch_rope(const RopeParams &p, int vec) {
-    const dim3 grid((p.rows + p.tokens - 1) / p.tokens), block(kRopeThreads);
-    if (vec == 8) launch_pdl(rope_kernel<T, 8>, grid, block, 0, p);
-    else if (vec == 4) launch_pdl(rope_kernel<T, 4>, grid, block, 0, p);
-    else if (vec == 2) launch_pdl(rope_kernel<T, 2>, grid, block, 0, p);
-    else launch_pdl(rope_kernel<T, 1>, grid, block, 0, p);
+    const dim3 grid((unsigned)((p.rows + (long long)p.grid.rows - 1) / p.grid.rows), p.grid.splits), block(p.grid.threads);
+    if constexpr (sizeof(T) == 2)
+        if (vec == 8) {
+            launch_pdl(rope_kernel<T, 8, INTER>, grid, block, 0, p);
+            return;
+        }
+    if (vec == 4) launch_pdl(rope_kernel<T, 4, INTER>, grid, block, 0, p);
+    else if (vec == 2) launch_pdl(rope_kernel<T, 2, INTER>, grid, block, 0, p);
+    else launch_pdl(rope_kernel<T, 1, INTER>, grid, block, 0, p);
 }
 
 }  // namespace
@@ -129,7 +138,7 @@ int rope_dev(int x_id, int x_off, int x_ld, int y_id, int y_off, int y_ld, int p
                                       {table_id, (size_t)rot_dim + 2, "table"}}))
         return rc;
     if (!rows) return kOk;
-    const int vec = rope_vector(head_dim, rot_dim, {x_off, y_off, x_ld, y_ld});
+    const int vec = rope_vector(type == kF32 ? 4 : 8, head_dim, rot_dim, interleaved, {x_off, y_off, x_ld, y_ld});
     RopeParams p;
     p.x = reinterpret_cast<const char *>(ptr(x_id)) + (size_t)x_off * elem_size(type);
     p.y = reinterpret_cast<char *>(ptr(y_id)) + (size_t)y_off * elem_size(type);
@@ -139,17 +148,17 @@ int rope_dev(int x_id, int x_off, int x_ld, int y_id, int y_off, int y_ld, int p
     p.y_ld = y_ld;
     p.rows = rows;
     p.shape = rope_shape(head_dim, rot_dim, interleaved != 0, vec);
-    const int per_row = heads * p.shape.units;
-    // a block takes rows until its threads have four units each, as long as every SM still gets two blocks
-    int tokens = 1;
-    while (tokens < kRopeTokens && tokens * per_row < 4 * kRopeThreads && rows / (2 * tokens) >= 2 * sm_count()) tokens *= 2;
-    p.tokens = tokens;
-    p.per_row = FastDiv(per_row);
-    p.per_head = FastDiv(p.shape.units);
+    p.heads = heads;
+    p.grid = rope_grid(rows, heads, p.shape.units);
     p.sign = inverse ? -1.0f : 1.0f;
-    if (type == kF32) launch_rope<float>(p, vec);
-    else if (type == kBf16) launch_rope<__nv_bfloat16>(p, vec);
-    else launch_rope<__half>(p, vec);
+    auto launch = [&](auto kind) {
+        using T = decltype(kind);
+        if (interleaved) launch_rope<T, true>(p, vec);
+        else launch_rope<T, false>(p, vec);
+    };
+    if (type == kF32) launch(float());
+    else if (type == kBf16) launch(__nv_bfloat16());
+    else launch(__half());
     ZB_LAUNCH_CHECK(name);
     return kOk;
 }

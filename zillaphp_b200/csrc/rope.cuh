@@ -14,67 +14,94 @@ namespace zb {
 
 struct RopeShape {
     int head_dim, rot, interleaved;
-    int pair_units, units;   // rotated units and all units of a head: a rotated one is two vectors, a copied one is one
+    int pair_units, units;   // rotated units and all units of a head
 };
 
-// Shared-memory (cos, sin) of `tokens` tokens' pairs: cs[token * rot/2 + pair].  pos[token] comes from
-// shared memory; sign -1 turns back.
-__device__ __forceinline__ void rope_angles(float2 *cs, const int *pos, int tokens, int half_rot,
-                                            const double *__restrict__ table, float sign, int tid, int threads) {
-    const float m = (float)table[half_rot];
-    for (int k = tid; k < tokens * half_rot; k += threads) {
-        const int t = k / half_rot, i = k - t * half_rot;
-        const double turns = (double)pos[t] * table[i];
-        const float f = (float)(turns - rint(turns));
-        float s, c;
-        sincospif(2.0f * f, &s, &c);
-        cs[k] = make_float2(m * c, m * sign * s);
-    }
+// A head's row is cut into units.  A rotated unit is two vectors with V pairs between them (half layout, and single
+// elements) or one vector that holds V / 2 pairs (interleaved), so that a warp's accesses stay contiguous; the
+// rest of the head is units of one vector that are copied.
+template <int V, bool INTER>
+struct RopeForm {
+    static constexpr bool kTwo = !INTER || V == 1;
+    static constexpr int kPairs = kTwo ? V : V / 2;
+    // Units that a thread loads before it finishes one: 128 bytes of 16-byte vectors, which with three blocks of
+    // 256 threads keeps 96 KB an SM on the way (HBM's 44 bytes a nanosecond and SM times two microseconds).
+    static constexpr int kBatch = kTwo ? 4 : 8;
+};
+
+// Where unit u's vectors lie in a head; y -1: one vector only.
+template <int V, bool INTER>
+__device__ __forceinline__ int2 rope_places(int u, const RopeShape &r) {
+    if (u >= r.pair_units) return make_int2(r.rot + (u - r.pair_units) * V, -1);
+    if (INTER) return V > 1 ? make_int2(u * V, -1) : make_int2(2 * u, 2 * u + 1);
+    return make_int2(u * V, (r.rot >> 1) + u * V);
 }
 
-// One unit of a head: u < pair_units turns V pairs, the rest copy V elements.  Everything is loaded
-// before anything is stored, so dst may be src.
-template <typename TI, typename TO, int V>
-__device__ __forceinline__ void rope_unit(const TI *src, TO *dst, const float2 *cs, int u, const RopeShape &r) {
-    if (u < r.pair_units) {
-        const int a_at = r.interleaved ? 2 * u * V : u * V, b_at = r.interleaved ? a_at + V : (r.rot >> 1) + u * V;
-        float a[V], b[V], x[V], y[V];
-        load_vec<TI, V>(src + a_at, a);
-        load_vec<TI, V>(src + b_at, b);
-        const float2 *c = cs + u * V;   // the unit's pairs are u V .. u V + V - 1 in both layouts
-        if (r.interleaved && V > 1) {
+// One unit's vectors as loaded.  A thread loads several units before it finishes one; a unit is stored after its
+// own loads, so dst may be src.
+template <typename TI, int V, bool TWO>
+struct RopeUnit {
+    RawVec<TI, V> a, b;
+    __device__ __forceinline__ void load(const TI *src, int2 at) {
+        a = load_raw<TI, V>(src + at.x);
+        if (TWO && at.y >= 0) b = load_raw<TI, V>(src + at.y);
+    }
+};
+
+// A thread's unit of every head that it takes: where it lies and its pairs' cosines and sines, which are the same for
+// all heads of a row, so they stay in registers.
+template <int V, bool INTER>
+struct RopeLane {
+    using Form = RopeForm<V, INTER>;
+    int2 at;
+    bool turns;        // a rotated unit (copied otherwise)
+    float co[Form::kPairs], si[Form::kPairs];
+    __device__ __forceinline__ void place(int u, const RopeShape &r) {
+        at = rope_places<V, INTER>(u, r);
+        turns = u < r.pair_units;
+    }
+    __device__ __forceinline__ void angles(int u, int pos, const RopeShape &r, const double *__restrict__ table, float sign) {
+        if (!turns) return;
+        const float m = (float)table[r.rot >> 1];
 #pragma unroll
-            for (int e = 0; e < V / 2; ++e) {
-                const float2 p = c[e], q = c[V / 2 + e];
-                x[2 * e] = a[2 * e] * p.x - a[2 * e + 1] * p.y;
-                x[2 * e + 1] = a[2 * e] * p.y + a[2 * e + 1] * p.x;
-                y[2 * e] = b[2 * e] * q.x - b[2 * e + 1] * q.y;
-                y[2 * e + 1] = b[2 * e] * q.y + b[2 * e + 1] * q.x;
-            }
-        } else {
+        for (int e = 0; e < Form::kPairs; ++e) {
+            const double t = (double)pos * table[u * Form::kPairs + e];
+            float s, c;
+            sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+            co[e] = m * c;
+            si[e] = m * sign * s;
+        }
+    }
+    static __device__ __forceinline__ void turn(float &x, float &y, float c, float s) {
+        const float t = x;
+        x = t * c - y * s;
+        y = t * s + y * c;
+    }
+    template <typename TI, typename TO>
+    __device__ __forceinline__ void finish(const RopeUnit<TI, V, Form::kTwo> &unit, TO *dst, bool rotate) const {
+        float x[V], y[V];
+        widen<TI, V>(unit.a, x);
+        if (Form::kTwo && at.y >= 0) widen<TI, V>(unit.b, y);
+        if (rotate && turns) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float2 p = c[e];
-                x[e] = a[e] * p.x - b[e] * p.y;
-                y[e] = a[e] * p.y + b[e] * p.x;
+            for (int e = 0; e < Form::kPairs; ++e) {
+                if (Form::kTwo) turn(x[e], y[e], co[e], si[e]);
+                else turn(x[2 * e], x[(2 * e + 1) % V], co[e], si[e]);
             }
         }
-        store_vec<TO, V>(dst + a_at, x);
-        store_vec<TO, V>(dst + b_at, y);
-    } else {
-        const int at = r.rot + (u - r.pair_units) * V;
-        float a[V];
-        load_vec<TI, V>(src + at, a);
-        store_vec<TO, V>(dst + at, a);
+        store_vec<TO, V>(dst + at.x, x);
+        if (Form::kTwo && at.y >= 0) store_vec<TO, V>(dst + at.y, y);
     }
-}
+};
 
-// The widest vector (8, 4, 2 or 1 elements) that divides a head's halves, its copied rest and every
-// offset and row stride of the call: 8 moves 16 bytes of a 16-bit type in one access.
-inline int rope_vector(int head_dim, int rot, std::initializer_list<long long> also) {
-    long long all = (long long)head_dim | (rot / 2);
+// The widest vector (`widest`, 16 bytes of the input's type, or less: 4, 2, 1 elements) that divides a head's halves (interleaved: its rotated part), its copied rest and every
+// offset and row stride of the call.
+inline int rope_vector(int widest, int head_dim, int rot, int interleaved, std::initializer_list<long long> also) {
+    long long all = (long long)head_dim | (interleaved ? rot : rot / 2);
     for (long long a : also) all |= a;
-    return all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+    for (int v = widest; v > 1; v /= 2)
+        if (all % v == 0) return v;
+    return 1;
 }
 
 inline RopeShape rope_shape(int head_dim, int rot, int interleaved, int vec) {
@@ -82,11 +109,33 @@ inline RopeShape rope_shape(int head_dim, int rot, int interleaved, int vec) {
     r.head_dim = head_dim;
     r.rot = rot;
     r.interleaved = interleaved;
-    r.pair_units = rot / 2 / vec;
+    r.pair_units = rot / 2 / (interleaved && vec > 1 ? vec / 2 : vec);
     r.units = r.pair_units + (head_dim - rot) / vec;
     return r;
 }
 
 constexpr int kRopeMaxDim = 256;
+constexpr int kRopeThreads = 256;
+constexpr int kRopeBlocks = 3;       // blocks an SM at least (80 registers a thread)
+
+// How threads share the work: a thread takes one unit of a row for heads h, h + lanes * splits, ...  A block is
+// rows x lanes x units (units fastest, so a warp reads along a head).  Heads are spread over as many threads as it
+// takes to fill the machine twice (two times 1024 threads an SM), and no more: each thread works out its pairs' angles.
+struct RopeGrid {
+    int rows, lanes, splits, threads;
+};
+inline RopeGrid rope_grid(long long rows, int heads, int units) {
+    RopeGrid g;
+    const long long want = 2048LL * sm_count(), have = rows * units;
+    long long spread = (want + have - 1) / have;
+    if (spread > heads) spread = heads;
+    const int room = kRopeThreads / units;   // units are 256 at most
+    g.lanes = (int)(spread < room ? spread : room);
+    g.splits = (int)((spread + g.lanes - 1) / g.lanes);
+    g.rows = room / g.lanes;
+    if (g.rows > rows) g.rows = (int)rows;
+    g.threads = (g.rows * g.lanes * units + 31) / 32 * 32;
+    return g;
+}
 
 }  // namespace zb
