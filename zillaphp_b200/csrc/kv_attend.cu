@@ -44,8 +44,17 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
         *abort_flag = 0;
         fence_barrier_init();
     }
+    // Behind the tcgen05 kernel nothing here depends on that kernel's results, and it has been started only after all blocks of
+    // it found the work before them done (they wait, then allow this one): the two run side by side.  What the host's
+    // earlier kernels wrote is read past L1 (__ldcg, TMA).  The last block only waits for
+    // the tcgen05 kernel, so that this grid does not end before it: the join behind waits for this grid alone.
     griddep_launch();
-    griddep_wait();
+    if (!p.behind_tc) {
+        griddep_wait();
+    } else if (blockIdx.x == gridDim.x - 1) {
+        griddep_wait();
+        return;
+    }
 
     // the block's item: (slot, row tile, kv head) of the prefix or of one sequence
     int item = blockIdx.x;
@@ -110,8 +119,8 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
                                                                  ((size_t)(first + j) * p.q_heads + (real ? hq : 0)) * D + c2);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-            qf[k][i] = real ? src[8 * k] : 0u;
-            qf[k][i + 2] = real ? src[8 * k + 4] : 0u;
+            qf[k][i] = real ? __ldcg(src + 8 * k) : 0u;
+            qf[k][i + 2] = real ? __ldcg(src + 8 * k + 4) : 0u;
         }
     }
     float o[D / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -283,19 +292,25 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     load_sequence(p, b, first, n, len);
     if (n == 0) return;
     const int own = (min(len, own_limit(len, n, t - first)) + p.own_chunk - 1) / p.own_chunk;
-    const int slots = p.prefix_splits + own;   // the prefix's come first and are there for every row
+    int front = p.prefix_splits;   // the prefix's slots come first
+    if (p.tc_blocks) {
+        const int hq = (int)(unit - (long long)t * p.q_heads), row = t * p.group + hq % p.group;
+        front = prefix_cut(p.batch.prefix_len, p.kv_heads * p.prefix_tiles, p.tc_blocks).slots(hq / p.group * p.prefix_tiles + row / (2 * kTcTile));
+    }
+    const int slots = front + own, skip = p.prefix_splits - front;   // the own ones lie behind the most that the prefix can have
     float m = -INFINITY;
-    for (int s = lane; s < slots; s += 32) m = fmaxf(m, p.part_ml[s * units + unit].x);
+    for (int s = lane; s < slots; s += 32) m = fmaxf(m, p.part_ml[(s < front ? s : s + skip) * units + unit].x);
 #pragma unroll
     for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
     if (m == -INFINITY) m = 0.0f;
     float acc[C] = {}, l = 0.0f;
 #pragma unroll 4
     for (int s = 0; s < slots; ++s) {
-        const float2 ml = p.part_ml[s * units + unit];
+        const long long at = (s < front ? s : s + skip) * units + unit;
+        const float2 ml = p.part_ml[at];
         const float w = ex2(ml.x - m);
         float v[C];
-        load_vec<float, C>(p.part_o + (s * units + unit) * D + lane * C, v);
+        load_vec<float, C>(p.part_o + at * D + lane * C, v);
         l += w * ml.y;
 #pragma unroll
         for (int i = 0; i < C; ++i) acc[i] += w * v[i];
@@ -308,7 +323,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
 
 // ---------------------------------------------------------------- plan
 struct Plan {
-    bool tc;                // the prefix on tcgen05
+    int tc_blocks;          // > 0: the prefix on tcgen05, by this many blocks
     int own_wm, prefix_wm;
     int own_tiles, prefix_tiles, own_chunk, own_splits, prefix_chunk, prefix_splits;
     bool direct;
@@ -320,40 +335,54 @@ int row_warps(long long rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 // Rows that share the prefix's keys from which it goes to tcgen05.
 constexpr int kTcRows = 64;
 
+// Blocks of the tcgen05 kernel.  It takes whole SMs (one block each) and is bound by the tensor cores and the softmax, the own
+// keys' kernel behind it by HBM, and runs on the SMs that are left; so with n blocks the call takes about
+//   t = units / n * tile + start,  plus what the other SMs - n have not moved by then at the whole machine's rate,
+// and n minimises that.  Measured: a tile of 256 rows and 128 keys 2.4 us with head_dim 128, 2.1 below; an SM alone draws about
+// 85 GB/s, all together 5.8 TB/s.  Lengths are on the device: half of their bound is assumed.
+int choose_tc_blocks(const KvCache &c, long long units, double own_bytes) {
+    const int sms = sm_count();
+    const double tile = c.head_dim == 128 ? 2.4e-6 : 2.1e-6, start = 6e-6, one = 85e9, all = 5.8e12;
+    int best = 1;
+    double least = 1e30;
+    for (int n = (int)std::min<long long>(units, sms); n >= 1 && n >= sms / 8; --n) {
+        const double t = (double)((units + n - 1) / n) * tile + start, left = std::max(0.0, own_bytes - (sms - n) * one * t);
+        if (t + left / all < least) {
+            least = t + left / all;
+            best = n;
+        }
+    }
+    return best;
+}
+
 // Row tiles of 16, 32 or 64 rows by the rows that share the keys, and slots of whole 64-key stages such
 // that all blocks together are about `kWaves` rounds of two blocks an SM: fewer would leave SMs idle, more would
-// add parts to write and join.  The tcgen05 kernel runs one block an SM: its slots minimise rounds x (tiles
-// of a block + kTcFixed tiles for its start and end).
+// add parts to write and join.
 Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_len, int max_new, int max_len) {
-    constexpr int kWaves = 2, kTcFixed = 3;
+    constexpr int kWaves = 2;
     Plan p;
     const int group = q_heads / c.kv_heads;
     const long long own_rows = (long long)max_new * group, prefix_rows = (long long)rows * group;
-    p.tc = prefix_rows > kTcRows && prefix_len > 0;
+    const bool tc = prefix_rows > kTcRows && prefix_len > 0;
     p.own_wm = row_warps(own_rows);
     p.prefix_wm = row_warps(prefix_rows);
     p.own_tiles = (int)((own_rows + 16 * p.own_wm - 1) / (16 * p.own_wm));
-    const int tile_rows = p.tc ? 2 * kTcTile : 16 * p.prefix_wm;
+    const int tile_rows = tc ? 2 * kTcTile : 16 * p.prefix_wm;
     p.prefix_tiles = (int)((prefix_rows + tile_rows - 1) / tile_rows);
     const long long own_steps = (max_len + kTile - 1) / kTile, prefix_steps = (prefix_len + kTile - 1) / kTile;
-    const long long total = c.kv_heads * (own_steps * batch * p.own_tiles + (p.tc ? 0 : prefix_steps * p.prefix_tiles));
+    const long long total = c.kv_heads * (own_steps * batch * p.own_tiles + (tc ? 0 : prefix_steps * p.prefix_tiles));
     const long long per = std::max<long long>(1, total / (2LL * kWaves * sm_count()));
     p.own_chunk = (int)std::min(per, std::max(1LL, own_steps)) * kTile;
     p.own_splits = (int)((max_len + p.own_chunk - 1) / p.own_chunk);
     p.prefix_chunk = (int)std::min(per, std::max(1LL, prefix_steps)) * kTile;
-    if (p.tc) {
-        const long long tiles = (prefix_len + kTcTile - 1) / kTcTile;
-        long long best = 0;
-        for (long long s = 1; s <= std::min(tiles, 64LL); ++s) {
-            const long long chunk = (tiles + s - 1) / s, slots = (tiles + chunk - 1) / chunk;
-            const long long rounds = (slots * p.prefix_tiles * c.kv_heads + sm_count() - 1) / sm_count(), cost = rounds * (chunk + kTcFixed);
-            if (s == 1 || cost < best) {
-                best = cost;
-                p.prefix_chunk = (int)chunk * kTcTile;
-            }
-        }
-    }
     p.prefix_splits = (int)(((long long)prefix_len + p.prefix_chunk - 1) / p.prefix_chunk);
+    p.tc_blocks = 0;
+    if (tc) {
+        const long long tiles = (prefix_len + kTcTile - 1) / kTcTile, units = tiles * c.kv_heads * p.prefix_tiles;
+        p.tc_blocks = choose_tc_blocks(c, units, 0.5 * 4.0 * batch * max_len * c.kv_heads * c.head_dim);
+        const long long each = units / p.tc_blocks;   // a block's units at least
+        p.prefix_splits = (int)std::min<long long>((tiles + each - 2) / each + 1, p.tc_blocks);
+    }
     if (p.own_splits + p.prefix_splits == 0) p.own_splits = 1;   // no keys at all: the rows are still written
     p.direct = p.own_splits == 1 && p.prefix_splits == 0;
     p.units = (size_t)rows * q_heads;
@@ -395,12 +424,13 @@ int run(AttendParams p, const Plan &plan, const char *name) {
     const long long own = (long long)p.batch.batch * p.own_splits * p.own_tiles * p.kv_heads;
     const long long prefix = (long long)p.prefix_splits * p.prefix_tiles * p.kv_heads;
     if (prefix > 0x7fffffffLL) return fail(kBadArg, "%s: %lld blocks are too many", name, prefix);
-    if (plan.tc) {
+    if (plan.tc_blocks) {
         static bool set[64] = {};
         if (int rc = allow_smem(attend_tc_kernel<T, D>, tc_smem<D>(), set, name)) return rc;
-        launch_pdl(attend_tc_kernel<T, D>, dim3((unsigned)prefix), dim3(kTcThreads), tc_smem<D>(), p);
+        launch_pdl(attend_tc_kernel<T, D>, dim3(plan.tc_blocks), dim3(kTcThreads), tc_smem<D>(), p);
         ZB_LAUNCH_CHECK(name);
-        if (int rc = run_split<T, D>(p, plan.own_wm, own, name)) return rc;
+        p.behind_tc = 1;
+        if (int rc = run_split<T, D>(p, plan.own_wm, own ? own + 1 : 0, name)) return rc;
     } else if (plan.own_wm == plan.prefix_wm) {
         p.prefix_items = (int)prefix;
         if (int rc = run_split<T, D>(p, plan.own_wm, prefix + own, name)) return rc;
@@ -499,6 +529,8 @@ int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int 
     p.prefix_tiles = plan.prefix_tiles;
     p.own_tiles = plan.own_tiles;
     p.prefix_items = 0;
+    p.tc_blocks = plan.tc_blocks;
+    p.behind_tc = 0;
     p.direct = plan.direct;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.err = device_error_word();

@@ -27,19 +27,40 @@ struct AttendParams {
     int prefix_splits, prefix_chunk, own_splits, own_chunk;   // slots, and keys of a slot
     int prefix_tiles, own_tiles;                              // row tiles of this launch
     int prefix_items;                                         // blocks [0, prefix_items) take the prefix
+    int tc_blocks;      // > 0: the prefix is cut evenly over this many blocks of the tcgen05 kernel
+    int behind_tc;      // the split kernel runs beside the tcgen05 kernel in front of it
     int direct;         // one slot in all: its kernel writes out itself
     float scale_log2;
     int *err;
 };
+
+// The tcgen05 kernel's cut of the prefix.  Its work is items (kv head, pair of row tiles) x key tiles of 128, item after
+// item; block c of n takes units [c U / n, (c + 1) U / n), so that no block has more than a tile over another, whatever the
+// counts.  An item's slots are the blocks that touch it, in order.
+struct PrefixCut {
+    long long units;
+    int tiles, blocks;
+    __host__ __device__ long long begin(int c) const { return c * units / blocks; }
+    __host__ __device__ int block_of(long long unit) const { return (int)(((unit + 1) * blocks - 1) / units); }
+    __host__ __device__ int first_block(int item) const { return block_of((long long)item * tiles); }
+    __host__ __device__ int slots(int item) const { return block_of((long long)(item + 1) * tiles - 1) - first_block(item) + 1; }
+};
+__host__ __device__ __forceinline__ PrefixCut prefix_cut(int prefix_len, int items, int blocks) {
+    PrefixCut c;
+    c.tiles = (prefix_len + 127) / 128;
+    c.units = (long long)items * c.tiles;
+    c.blocks = blocks;
+    return c;
+}
 
 // Keys that row j of a sequence sees of its own: clamped to 0 .. len.
 __device__ __forceinline__ int own_limit(int len, int n, int j) { return max(0, len - n + j + 1); }
 
 // A sequence's new rows and length; one that does not fit the call's sizes is recorded and has no rows.
 __device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int &first, int &n, int &len) {
-    first = p.batch.start[b];
-    n = p.batch.start[b + 1] - first;
-    len = p.batch.len[b];
+    first = __ldcg(p.batch.start + b);
+    n = __ldcg(p.batch.start + b + 1) - first;
+    len = __ldcg(p.batch.len + b);
     if (first < 0 || n < 0 || n > p.max_new || (long long)first + n > p.batch.rows || len < 0 || len > p.max_len) {
         atomicCAS(p.err, 0, kErrKvLength);
         n = 0;
@@ -52,7 +73,7 @@ __device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int 
 __device__ __forceinline__ int box_row(const AttendParams &p, const int *pages, int kv_head, int key, int end) {
     const int none = p.pages * p.kv_heads << p.page_log2;
     if (key >= end) return none;
-    const int id = pages[key >> p.page_log2];
+    const int id = __ldcg(pages + (key >> p.page_log2));
     if (id < 0 || id >= p.pages) {
         atomicCAS(p.err, 0, kErrKvPage);
         return none;

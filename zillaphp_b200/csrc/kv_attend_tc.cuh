@@ -1,8 +1,9 @@
 // kv_attend_tc.cuh -- the shared prefix's part of zilla_kv_attend on tcgen05, for batches whose rows
 // (tokens x query heads of a kv head) fill 128-row tiles.
 //
-// One block takes two 128-row tiles ("streams"), one kv head and one slot of the prefix's keys; both
-// streams use each K and V tile of 128 keys, so a tile crosses L2 once for 256 rows.  Per tile and stream:
+// An item is two 128-row tiles ("streams") of one kv head; both streams use each K and V tile of 128 keys, so a
+// tile crosses L2 once for 256 rows.  A block takes an even share of all items' key tiles (PrefixCut): parts of one to
+// a few items ("segments"), one after the other.  Per tile and stream:
 //   S = Q K^T          M = 128 rows, N = 128 keys, K = head_dim, fp32 in TMEM
 //   P = 2^(S - ref)    one thread a row; P (16 bits) replaces S in TMEM, two keys a column
 //   O += P V           A = P from TMEM, B = V [key][d] (N-major), N = head_dim, fp32 in TMEM
@@ -119,21 +120,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    int item = blockIdx.x;
-    const int pair = item % p.prefix_tiles;
-    item /= p.prefix_tiles;
-    const int head = item % p.kv_heads, slot = item / p.kv_heads;
-    const int rows = p.batch.rows * p.group, row0 = pair * 2 * kTcTile;
-    const int streams = rows - row0 > kTcTile ? 2 : 1;
-    const int begin = slot * p.prefix_chunk, end = min(begin + p.prefix_chunk, p.batch.prefix_len);
-    const int tiles = (end - begin + kTcTile - 1) / kTcTile;
+    const int rows = p.batch.rows * p.group;
+    const PrefixCut cut = prefix_cut(p.batch.prefix_len, p.kv_heads * p.prefix_tiles, p.tc_blocks);
+    const long long unit0 = cut.begin(blockIdx.x), unit1 = cut.begin(blockIdx.x + 1);
+    // the block's segments in order, the same in every role: fn(kv head, first row, streams, first tile, tiles, slot) until it returns false
+    auto segments = [&](auto fn) {
+        for (long long unit = unit0; unit < unit1;) {
+            const int item = (int)(unit / cut.tiles), tile0 = (int)(unit - (long long)item * cut.tiles);
+            const int tiles = (int)min((long long)(cut.tiles - tile0), unit1 - unit), row0 = item % p.prefix_tiles * 2 * kTcTile;
+            if (!fn(item / p.prefix_tiles, row0, rows - row0 > kTcTile ? 2 : 1, tile0, tiles, (int)blockIdx.x - cut.first_block(item))) return;
+            unit += tiles;
+        }
+    };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
         }
-        mbar_init(q_full, streams * kTcTile);
+        mbar_init(q_full, 2 * kTcTile);
         for (int s = 0; s < 2; ++s) {
             mbar_init(s_full + s, 1);
             mbar_init(p_full + s, kTcTile);
@@ -148,26 +153,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    griddep_launch();
     griddep_wait();
+    griddep_launch();   // behind the wait: a kernel started by it finds everything before this one done
 
     if (warp == 8) {
         // ---- loads: K and V tiles alternate through the ring
         const int boxes = kTcTile / p.box_rows, all = boxes * kHalves;   // 2 .. 16
         const int r0 = lane % boxes * p.box_rows, half = lane / boxes;
         bool ok = true;
-        int i = 0;
-        for (; i < 2 * tiles; ++i) {
-            const int st = i % ST;
-            const int at = lane < all ? box_row(p, p.prefix_pages, head, begin + (i >> 1) * kTcTile + r0, end) : 0;
-            ok = i < ST || mbar_wait(empty + st, (i / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(full + st, kTileBytes);
-            __syncwarp();
-            if (lane < all)
-                tma_load_2d(ring + st * kTileBytes + half * kHalfBytes + r0 * kRowBytes, i & 1 ? &p.v_map : &p.k_map, full + st, half * 64, at);
-        }
+        int i = 0;   // loads so far: K of a tile, then V
+        segments([&](int head, int, int, int tile0, int tiles, int) {
+            for (int x = 0; x < 2 * tiles; ++x, ++i) {
+                const int st = i % ST;
+                const int at = lane < all ? box_row(p, p.prefix_pages, head, (tile0 + (x >> 1)) * kTcTile + r0, p.batch.prefix_len) : 0;
+                ok = i < ST || mbar_wait(empty + st, (i / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return false;
+                if (lane == 0) mbar_arrive_expect_tx(full + st, kTileBytes);
+                __syncwarp();
+                if (lane < all)
+                    tma_load_2d(ring + st * kTileBytes + half * kHalfBytes + r0 * kRowBytes, x & 1 ? &p.v_map : &p.k_map, full + st, half * 64, at);
+            }
+            return true;
+        });
         if (!ok && lane == 0)   // the copies in flight end before the block's shared memory goes
             for (int x = max(0, i - ST); x < i; ++x)
                 if (!mbar_wait_drain(full + x % ST, (x / ST) & 1)) atomicCAS(p.err, 0, kErrDrain);
@@ -175,7 +183,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         // ---- MMAs
         if (lane == 0) {
             constexpr uint32_t kIdS = attend_idesc<T>(kTcTile, false), kIdO = attend_idesc<T>(D, true);
-            auto wait_tile = [&](int i) { return mbar_wait(full + i % ST, (i / ST) & 1, abort_flag, p.err, kErrFullWait); };
+            auto wait_load = [&](int i) { return mbar_wait(full + i % ST, (i / ST) & 1, abort_flag, p.err, kErrFullWait); };
             auto qk = [&](int s, int i) {
                 const uint32_t a = smem_u32(base) + s * kTileBytes, b = smem_u32(ring) + i % ST * kTileBytes;
 #pragma unroll
@@ -191,133 +199,145 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                 for (int k = 0; k < kTcTile / 16; ++k)
                     mma_f16_ta(tmem + 256 + s * D, tmem + s * 128 + 8 * k, smem_desc(b + k * 2 * kAtom, kHalfBytes, kAtom, kSw), kIdO, more || k != 0);
             };
-            bool ok = mbar_wait(q_full, 0, abort_flag, p.err, kErrFullWait) && wait_tile(0);
-            if (ok) {
+            bool ok = true;
+            int i = 0, done[2] = {0, 0}, segment = 0;   // loads taken, tiles of each stream, segments
+            segments([&](int, int, int streams, int, int tiles, int) {
+                ok = mbar_wait(q_full, segment++ & 1, abort_flag, p.err, kErrFullWait) && wait_load(i);
+                if (!ok) return false;
                 tc_fence_after();
-                for (int s = 0; s < streams; ++s) qk(s, 0);
-                mma_commit(empty);
-            }
-            for (int j = 0; ok && j < tiles; ++j) {
-                ok = wait_tile(2 * j + 1);
-                for (int s = 0; ok && s < streams; ++s) {
-                    ok = mbar_wait(p_full + s, j & 1, abort_flag, p.err, kErrAccWait);
-                    if (!ok) break;
-                    tc_fence_after();
-                    pv(s, 2 * j + 1, j > 0);
-                    if (j + 1 == tiles) {
-                        mma_commit(o_full + s);
-                    } else {
-                        ok = s > 0 || wait_tile(2 * j + 2);
+                for (int s = 0; s < streams; ++s) qk(s, i);
+                mma_commit(empty + i % ST);
+                for (int j = 0; j < tiles; ++j, i += 2) {
+                    ok = wait_load(i + 1);
+                    for (int s = 0; ok && s < streams; ++s) {
+                        ok = mbar_wait(p_full + s, done[s]++ & 1, abort_flag, p.err, kErrAccWait);
                         if (!ok) break;
                         tc_fence_after();
-                        qk(s, 2 * j + 2);
+                        pv(s, i + 1, j > 0);
+                        if (j + 1 == tiles) {
+                            mma_commit(o_full + s);
+                        } else {
+                            ok = s > 0 || wait_load(i + 2);
+                            if (!ok) break;
+                            tc_fence_after();
+                            qk(s, i + 2);
+                        }
                     }
+                    if (!ok) return false;
+                    mma_commit(empty + (i + 1) % ST);
+                    if (j + 1 < tiles) mma_commit(empty + (i + 2) % ST);
                 }
-                if (!ok) break;
-                mma_commit(empty + (2 * j + 1) % ST);
-                if (j + 1 < tiles) mma_commit(empty + (2 * j + 2) % ST);
-            }
+                return true;
+            });
             if (!ok) {   // MMAs in flight end before TMEM goes
                 mma_commit(drain);
                 if (!mbar_wait_drain(drain, 0)) atomicCAS(p.err, 0, kErrDrain);
             }
         }
         __syncwarp();
-    } else if (warp < 4 * streams) {
+    } else {
         // ---- softmax: thread = row of the stream
-        const int s = warp >> 2, r = threadIdx.x & (kTcTile - 1), row = row0 + s * kTcTile + r;
-        const bool real = row < rows;
-        const int t = real ? row / p.group : 0, hq = head * p.group + (real ? row - t * p.group : 0);
-        const size_t unit = (size_t)t * p.q_heads + hq;
-        {
-            // with a negative scale the queries change their sign, so that the largest product has the largest score
-            const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + unit * D);
-            const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                uint4 x = real ? src[c] : make_uint4(0, 0, 0, 0);
-                x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                *reinterpret_cast<uint4 *>(base + s * kTileBytes + tile_chunk<D>(r, c, kTcTile)) = x;
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(q_full);
-        }
+        const int s = warp >> 2, r = threadIdx.x & (kTcTile - 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + s * 128, to = tmem + lanes + 256 + s * D;
         const float sl = fmaxf(fabsf(p.scale_log2), 1e-30f);   // above zero: a masked -inf stays one
         const uint64_t sl2 = pack_f32x2(sl, sl);
-        float ref = 0.0f, l = 0.0f;   // ref in units of log2
-        bool ok = true;
-        for (int j = 0; j < tiles; ++j) {
-            ok = mbar_wait(s_full + s, j & 1, abort_flag, p.err, kErrAccWait);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            tc_fence_after();
-            uint32_t v[4][32];
+        int done = 0, loads = 0, segment = 0, mine = 0;   // tiles of this stream, loads of the ring, segments, this stream's segments
+        segments([&](int head, int row0, int streams, int tile0, int tiles, int slot) {
+            if (s >= streams) {   // no rows here; not to arrive for the next segment before this one's queries are there
+                mbar_arrive(q_full);
+                loads += 2 * tiles;
+                return __all_sync(0xffffffffu, mbar_wait(q_full, segment++ & 1, abort_flag, p.err, kErrAccWait)) != 0;
+            }
+            ++segment;
+            const int row = row0 + s * kTcTile + r;
+            const bool real = row < rows;
+            const int t = real ? row / p.group : 0, hq = head * p.group + (real ? row - t * p.group : 0);
+            const size_t unit = (size_t)t * p.q_heads + hq;
+            {
+                // with a negative scale the queries change their sign, so that the largest product has the largest score
+                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + unit * D);
+                const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32_async(ts + 32 * c, v[c]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld_wait(v[c]);
-            const int left = end - (begin + j * kTcTile);
-            if (left < kTcTile) {   // the last tile's missing keys; V behind them counts as zero, whatever its page holds
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (32 * c + i >= left) v[c][i] = 0xff800000u;
-                const int st = (2 * j + 1) % ST;
-                ok = mbar_wait(full + st, ((2 * j + 1) / ST) & 1, abort_flag, p.err, kErrFullWait);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                for (int x = r; x < (kTcTile - left) * (D / 8); x += kTcTile)
-                    *reinterpret_cast<uint4 *>(ring + st * kTileBytes + tile_chunk<D>(left + x / (D / 8), x % (D / 8), kTcTile)) = make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < D / 8; ++c) {
+                    uint4 x = real ? src[c] : make_uint4(0, 0, 0, 0);
+                    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                    *reinterpret_cast<uint4 *>(base + s * kTileBytes + tile_chunk<D>(r, c, kTcTile)) = x;
+                }
                 fence_proxy_async_smem();
+                mbar_arrive(q_full);
             }
-            float top[4];
+            float ref = 0.0f, l = 0.0f;   // ref in units of log2
+            for (int j = 0; j < tiles; ++j, loads += 2) {
+                bool ok = mbar_wait(s_full + s, done++ & 1, abort_flag, p.err, kErrAccWait);
+                if (!__all_sync(0xffffffffu, ok)) return false;
+                tc_fence_after();
+                uint32_t v[4][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                top[c] = __uint_as_float(v[c][0]);
+                for (int c = 0; c < 4; ++c) tmem_ld32_async(ts + 32 * c, v[c]);
 #pragma unroll
-                for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(v[c][i]));
-            }
-            float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
-            if (!(m > -INFINITY)) m = j ? ref : 0.0f;   // no key yet
-            if (j == 0) ref = m;
-            else if (__any_sync(0xffffffffu, m > ref + 8.0f)) {
-                const float f = m > ref ? ex2(ref - m) : 1.0f;
-                ref = fmaxf(ref, m);
-                l *= f;
+                for (int c = 0; c < 4; ++c) tmem_ld_wait(v[c]);
+                const int left = p.batch.prefix_len - (tile0 + j) * kTcTile;
+                if (left < kTcTile) {   // the last tile's missing keys; V behind them counts as zero, whatever its page holds
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32_async(to + 32 * c, o);
-                    tmem_ld_wait(o);
-                    uint32_t w[2][16];
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) w[i >> 4][i & 15] = __float_as_uint(__uint_as_float(o[i]) * f);
-                    tmem_st16(to + 32 * c, w[0]);
-                    tmem_st16(to + 32 * c + 16, w[1]);
+                        for (int i = 0; i < 32; ++i)
+                            if (32 * c + i >= left) v[c][i] = 0xff800000u;
+                    const int st = (loads + 1) % ST;
+                    ok = mbar_wait(full + st, ((loads + 1) / ST) & 1, abort_flag, p.err, kErrFullWait);
+                    if (!__all_sync(0xffffffffu, ok)) return false;
+                    for (int x = r; x < (kTcTile - left) * (D / 8); x += kTcTile)
+                        *reinterpret_cast<uint4 *>(ring + st * kTileBytes + tile_chunk<D>(left + x / (D / 8), x % (D / 8), kTcTile)) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
                 }
-            }
-            const uint64_t nref = pack_f32x2(-ref, -ref);
-            uint64_t sum[2] = {0, 0};
+                float top[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t w[16];
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = __uint_as_float(v[c][0]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sl2, nref));
-                    const float a = ex2(x.x), b = ex2(x.y);
-                    sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(a, b));
-                    w[i] = pack2<T>(a, b);
+                    for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(v[c][i]));
                 }
-                tmem_st16(ts + 16 * c, w);
+                float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
+                if (!(m > -INFINITY)) m = j ? ref : 0.0f;   // no key yet
+                if (j == 0) ref = m;
+                else if (__any_sync(0xffffffffu, m > ref + 8.0f)) {
+                    const float f = m > ref ? ex2(ref - m) : 1.0f;
+                    ref = fmaxf(ref, m);
+                    l *= f;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32_async(to + 32 * c, o);
+                        tmem_ld_wait(o);
+                        uint32_t w[2][16];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i >> 4][i & 15] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(to + 32 * c, w[0]);
+                        tmem_st16(to + 32 * c + 16, w[1]);
+                    }
+                }
+                const uint64_t nref = pack_f32x2(-ref, -ref);
+                uint64_t sum[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sl2, nref));
+                        const float a = ex2(x.x), b = ex2(x.y);
+                        sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(a, b));
+                        w[i] = pack2<T>(a, b);
+                    }
+                    tmem_st16(ts + 16 * c, w);
+                }
+                const float2 add = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+                l += add.x + add.y;
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(p_full + s);
             }
-            const float2 add = unpack_f32x2(add_f32x2(sum[0], sum[1]));
-            l += add.x + add.y;
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(p_full + s);
-        }
-        if (ok) ok = mbar_wait(o_full + s, 0, abort_flag, p.err, kErrAccWait);
-        if (__all_sync(0xffffffffu, ok)) {
+            bool ok = mbar_wait(o_full + s, mine++ & 1, abort_flag, p.err, kErrAccWait);
+            if (!__all_sync(0xffffffffu, ok)) return false;
             tc_fence_after();
             const size_t at = (size_t)slot * p.batch.rows * p.q_heads + unit;
             float4 *dst = reinterpret_cast<float4 *>(p.part_o + at * D);
@@ -333,7 +353,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                                                      __uint_as_float(o[4 * i + 3]));
             }
             if (real) p.part_ml[at] = make_float2(ref, l);
-        }
+            tc_fence_before();
+            return true;
+        });
     }
     tc_fence_before();
     __syncthreads();
