@@ -4,18 +4,20 @@
 // An item is two 128-row tiles ("streams") of one kv head; both streams use each K and V tile of 128 keys, so a
 // tile crosses L2 once for 256 rows.  A block takes an even share of all items' key tiles (PrefixCut): parts of one to
 // a few items ("segments"), one after the other.  Per tile and stream:
-//   S = Q K^T          M = 128 rows, N = 128 keys, K = head_dim, fp32 in TMEM
+// in two steps of 64 keys:
+//   S = Q K^T          M = 128 rows, N = 64 keys, K = head_dim, fp32 in TMEM
 //   P = 2^(S - ref)    one thread a row; P (16 bits) replaces S in TMEM, two keys a column
-//   O += P V           A = P from TMEM, B = V [key][d] (N-major), N = head_dim, fp32 in TMEM
+//   O += P V           A = P from TMEM, B = V [key][d] (N-major), N = head_dim, K = 64 keys, fp32 in TMEM
+// A stream has two S buffers of 64 columns, so that S of the next step is there when P of this one is done: the softmax
+// never waits for an MMA of its own stream.  (One buffer of 128 keys makes softmax, P V and Q K^T a chain: 2.4 us a
+// tile against the 1.6 us of this form.)
 // ref is the row's maximum as of its last change: it follows the true maximum only when that has passed it
 // by 2^8 (then O and l are rescaled), so that O rarely has to travel through registers; weights stay
 // below 2^8 and l and O carry the same factor, so the quotient does not change.
-// Warps 0-3 and 4-7 are the streams' softmax, warp 8 loads (TMA through the page list), warp 9 issues the
-// MMAs: while one stream's softmax runs, the other's MMAs do.
+// Warps 0-3 and 4-7 are the streams' softmax, warp 8 loads (TMA through the page list), warp 9 issues the MMAs.
 //
-// Order of the MMAs of a stream: P V of tile j, then Q K^T of tile j + 1 over the same TMEM columns; one
-// thread issues both and the tensor pipe takes them in order.  S's barrier of tile j + 1 is a commit behind
-// P V of tile j, so a softmax that sees it may also rescale O.
+// Order of a stream's MMAs: P V of step h, then Q K^T of step h + 2 over the same TMEM columns; one thread
+// issues both and the tensor pipe takes them in order.
 #pragma once
 
 #include "kv_attend.cuh"
@@ -26,6 +28,7 @@ namespace kv {
 using namespace tc;
 
 constexpr int kTcTile = 128;      // rows of a stream, keys of a tile
+constexpr int kTcStep = 64;       // keys of a step
 constexpr int kTcThreads = 320;
 
 template <int D>
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
     uint8_t *base = smem_raw + (((raw + 1023u) & ~1023u) - raw);    // Q of both streams, then the ring
     uint8_t *ring = base + 2 * kTileBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + ST * kTileBytes);
-    uint64_t *full = bars, *empty = bars + ST, *q_full = bars + 2 * ST, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 2, *drain = o_full + 2;
+    uint64_t *full = bars, *empty = bars + ST, *q_full = bars + 2 * ST, *s_full = q_full + 1, *p_full = s_full + 4, *o_done = p_full + 4, *drain = o_done + 4;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -139,10 +142,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             mbar_init(empty + i, 1);
         }
         mbar_init(q_full, 2 * kTcTile);
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(s_full + s, 1);
-            mbar_init(p_full + s, kTcTile);
-            mbar_init(o_full + s, 1);
+        for (int i = 0; i < 4; ++i) {   // [stream][step & 1]: a waiter is at most one phase behind
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, kTcTile);
+            mbar_init(o_done + i, 1);
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -180,68 +183,104 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             for (int x = max(0, i - ST); x < i; ++x)
                 if (!mbar_wait_drain(full + x % ST, (x / ST) & 1)) atomicCAS(p.err, 0, kErrDrain);
     } else if (warp == 9) {
-        // ---- MMAs
-        if (lane == 0) {
-            constexpr uint32_t kIdS = attend_idesc<T>(kTcTile, false), kIdO = attend_idesc<T>(D, true);
-            auto wait_load = [&](int i) { return mbar_wait(full + i % ST, (i / ST) & 1, abort_flag, p.err, kErrFullWait); };
-            auto qk = [&](int s, int i) {
-                const uint32_t a = smem_u32(base) + s * kTileBytes, b = smem_u32(ring) + i % ST * kTileBytes;
+        // ---- MMAs.  The whole warp runs the loop, one elected lane issues: addresses stay in uniform registers, and a
+        // step's twelve MMAs follow each other without work between them.
+        constexpr uint32_t kIdS = attend_idesc<T>(kTcStep, false), kIdO = attend_idesc<T>(D, true);
+        constexpr uint32_t kStep16 = kTcStep * kRowBytes / 16, kTile16 = kTileBytes / 16;   // in the descriptors' units of 16 bytes
+        const uint64_t q_desc = smem_desc(smem_u32(base), 16, kAtom, kSw), k_desc = smem_desc(smem_u32(ring), 16, kAtom, kSw),
+                       v_desc = smem_desc(smem_u32(ring), kHalfBytes, kAtom, kSw);
+        struct Place {   // a load's place in the ring
+            int st = 0, turn = 0;
+            __device__ __forceinline__ void next() {
+                if (++st == ST) {
+                    st = 0;
+                    turn ^= 1;
+                }
+            }
+        };
+        auto wait_load = [&](const Place &x) { return mbar_wait(full + x.st, x.turn, abort_flag, p.err, kErrFullWait); };
+        auto qk = [&](int s, int h, int st) {   // step h of the segment, whose K is in stage st
+            const uint64_t a = q_desc + s * kTile16, b = k_desc + st * kTile16 + (h & 1) * kStep16;
+            const uint32_t d = tmem + s * 128 + (h & 1) * kTcStep;
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t at = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    mma_bf16(tmem + s * 128, smem_desc(a + at, 16, kAtom, kSw), smem_desc(b + at, 16, kAtom, kSw), kIdS, k != 0);
+                    const uint32_t at = ((k >> 2) * kHalfBytes + (k & 3) * 32) / 16;
+                    mma_bf16(d, a + at, b + at, kIdS, k != 0);
                 }
-                mma_commit(s_full + s);
-            };
-            auto pv = [&](int s, int i, bool more) {
-                const uint32_t b = smem_u32(ring) + i % ST * kTileBytes;
+                mma_commit(s_full + 2 * s + (h & 1));
+            }
+            __syncwarp();
+        };
+        auto pv = [&](int s, int h, int st, bool last) {
+            const uint64_t b = v_desc + st * kTile16 + (h & 1) * kStep16;
+            const uint32_t a = tmem + s * 128 + (h & 1) * kTcStep, d = tmem + 256 + s * D;
+            if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kTcTile / 16; ++k)
-                    mma_f16_ta(tmem + 256 + s * D, tmem + s * 128 + 8 * k, smem_desc(b + k * 2 * kAtom, kHalfBytes, kAtom, kSw), kIdO, more || k != 0);
-            };
-            bool ok = true;
-            int i = 0, done[2] = {0, 0}, segment = 0;   // loads taken, tiles of each stream, segments
-            segments([&](int, int, int streams, int, int tiles, int) {
-                ok = mbar_wait(q_full, segment++ & 1, abort_flag, p.err, kErrFullWait) && wait_load(i);
-                if (!ok) return false;
-                tc_fence_after();
-                for (int s = 0; s < streams; ++s) qk(s, i);
-                mma_commit(empty + i % ST);
-                for (int j = 0; j < tiles; ++j, i += 2) {
-                    ok = wait_load(i + 1);
+                for (int k = 0; k < kTcStep / 16; ++k) mma_f16_ta(d, a + 8 * k, b + k * (2 * kAtom / 16), kIdO, h > 0 || k != 0);
+                if (last) mma_commit(o_done + 2 * s + (h & 1));
+            }
+            __syncwarp();
+        };
+        auto release = [&](int st) {
+            if (elect_one()) mma_commit(empty + st);
+            __syncwarp();
+        };
+        bool ok = true;
+        int done[2] = {0, 0}, segment = 0;   // pairs of steps of each stream, segments
+        Place k_at, v_at;                    // the tile's K and V
+        v_at.next();
+        segments([&](int, int, int streams, int, int tiles, int) {
+            ok = mbar_wait(q_full, segment++ & 1, abort_flag, p.err, kErrFullWait) && wait_load(k_at);
+            if (!ok) return false;
+            tc_fence_after();
+            for (int h = 0; h < 2; ++h)
+                for (int s = 0; s < streams; ++s) qk(s, h, k_at.st);
+            release(k_at.st);
+            for (int j = 0; j < tiles; ++j) {
+                const bool more = j + 1 < tiles;
+                k_at.next();
+                k_at.next();
+                ok = wait_load(v_at);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
                     for (int s = 0; ok && s < streams; ++s) {
-                        ok = mbar_wait(p_full + s, done[s]++ & 1, abort_flag, p.err, kErrAccWait);
+                        ok = mbar_wait(p_full + 2 * s + h, done[s] & 1, abort_flag, p.err, kErrAccWait);
                         if (!ok) break;
                         tc_fence_after();
-                        pv(s, i + 1, j > 0);
-                        if (j + 1 == tiles) {
-                            mma_commit(o_full + s);
-                        } else {
-                            ok = s > 0 || wait_load(i + 2);
-                            if (!ok) break;
-                            tc_fence_after();
-                            qk(s, i + 2);
+                        pv(s, 2 * j + h, v_at.st, !more);
+                        if (more) {
+                            if (h == 0 && s == 0) {
+                                ok = wait_load(k_at);
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            qk(s, h, k_at.st);
                         }
+                        done[s] += h;
                     }
-                    if (!ok) return false;
-                    mma_commit(empty + (i + 1) % ST);
-                    if (j + 1 < tiles) mma_commit(empty + (i + 2) % ST);
-                }
-                return true;
-            });
-            if (!ok) {   // MMAs in flight end before TMEM goes
+                if (!ok) return false;
+                release(v_at.st);
+                if (more) release(k_at.st);
+                v_at.next();
+                v_at.next();
+            }
+            return true;
+        });
+        if (!ok) {   // MMAs in flight end before TMEM goes
+            if (elect_one()) {
                 mma_commit(drain);
                 if (!mbar_wait_drain(drain, 0)) atomicCAS(p.err, 0, kErrDrain);
             }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // ---- softmax: thread = row of the stream
         const int s = warp >> 2, r = threadIdx.x & (kTcTile - 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + s * 128, to = tmem + lanes + 256 + s * D;
         const float sl = fmaxf(fabsf(p.scale_log2), 1e-30f);   // above zero: a masked -inf stays one
         const uint64_t sl2 = pack_f32x2(sl, sl);
-        int done = 0, loads = 0, segment = 0, mine = 0;   // tiles of this stream, loads of the ring, segments, this stream's segments
+        int done = 0, loads = 0, segment = 0, mine = 0;   // steps of this stream, loads of the ring, segments, this stream's segments
         segments([&](int head, int row0, int streams, int tile0, int tiles, int slot) {
             if (s >= streams) {   // no rows here; not to arrive for the next segment before this one's queries are there
                 mbar_arrive(q_full);
@@ -267,40 +306,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                 mbar_arrive(q_full);
             }
             float ref = 0.0f, l = 0.0f;   // ref in units of log2
-            for (int j = 0; j < tiles; ++j, loads += 2) {
-                bool ok = mbar_wait(s_full + s, done++ & 1, abort_flag, p.err, kErrAccWait);
+            for (int h = 0; h < 2 * tiles; ++h, ++done) {
+                const int buf = h & 1;
+                bool ok = mbar_wait(s_full + 2 * s + buf, (done >> 1) & 1, abort_flag, p.err, kErrAccWait);
                 if (!__all_sync(0xffffffffu, ok)) return false;
                 tc_fence_after();
-                uint32_t v[4][32];
+                uint32_t v[2][32];
+                tmem_ld32_async(ts + buf * kTcStep, v[0]);
+                tmem_ld32_async(ts + buf * kTcStep + 32, v[1]);
+                tmem_ld_wait(v[0]);
+                tmem_ld_wait(v[1]);
+                const int left = p.batch.prefix_len - tile0 * kTcTile - h * kTcStep;   // keys from this step's first on
+                if (left < kTcTile) {
+                    if (left < kTcStep) {   // the missing keys
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32_async(ts + 32 * c, v[c]);
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_wait(v[c]);
-                const int left = p.batch.prefix_len - (tile0 + j) * kTcTile;
-                if (left < kTcTile) {   // the last tile's missing keys; V behind them counts as zero, whatever its page holds
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (32 * c + i >= left) v[c][i] = 0xff800000u;
-                    const int st = (loads + 1) % ST;
-                    ok = mbar_wait(full + st, ((loads + 1) / ST) & 1, abort_flag, p.err, kErrFullWait);
-                    if (!__all_sync(0xffffffffu, ok)) return false;
-                    for (int x = r; x < (kTcTile - left) * (D / 8); x += kTcTile)
-                        *reinterpret_cast<uint4 *>(ring + st * kTileBytes + tile_chunk<D>(left + x / (D / 8), x % (D / 8), kTcTile)) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
+                            for (int i = 0; i < 32; ++i)
+                                if (32 * c + i >= left) v[c][i] = 0xff800000u;
+                    }
+                    if (!buf) {   // V behind the last key counts as zero, whatever its page holds
+                        const int load = loads + h + 1, st = load % ST;
+                        ok = mbar_wait(full + st, (load / ST) & 1, abort_flag, p.err, kErrFullWait);
+                        if (!__all_sync(0xffffffffu, ok)) return false;
+                        for (int x = r; x < (kTcTile - left) * (D / 8); x += kTcTile)
+                            *reinterpret_cast<uint4 *>(ring + st * kTileBytes + tile_chunk<D>(left + x / (D / 8), x % (D / 8), kTcTile)) =
+                                make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                    }
                 }
                 float top[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    top[c] = __uint_as_float(v[c][0]);
+                    top[c] = __uint_as_float(v[c >> 1][(c & 1) * 16]);
 #pragma unroll
-                    for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(v[c][i]));
+                    for (int i = 1; i < 16; ++i) top[c] = fmaxf(top[c], __uint_as_float(v[c >> 1][(c & 1) * 16 + i]));
                 }
                 float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
-                if (!(m > -INFINITY)) m = j ? ref : 0.0f;   // no key yet
-                if (j == 0) ref = m;
+                if (!(m > -INFINITY)) m = h ? ref : 0.0f;   // no key yet
+                if (h == 0) ref = m;
                 else if (__any_sync(0xffffffffu, m > ref + 8.0f)) {
+                    // O with the step before in it: S of the next step is committed behind that, or the segment's last steps themselves
+                    ok = h + 1 < 2 * tiles ? mbar_wait(s_full + 2 * s + (buf ^ 1), ((done + 1) >> 1) & 1, abort_flag, p.err, kErrAccWait)
+                                           : mbar_wait(o_done + 2 * s + (buf ^ 1), mine & 1, abort_flag, p.err, kErrAccWait);
+                    if (!__all_sync(0xffffffffu, ok)) return false;
+                    tc_fence_after();
                     const float f = m > ref ? ex2(ref - m) : 1.0f;
                     ref = fmaxf(ref, m);
                     l *= f;
@@ -319,7 +369,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                 const uint64_t nref = pack_f32x2(-ref, -ref);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -328,15 +378,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                         sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(a, b));
                         w[i] = pack2<T>(a, b);
                     }
-                    tmem_st16(ts + 16 * c, w);
+                    tmem_st16(ts + buf * kTcStep + 16 * c, w);
                 }
                 const float2 add = unpack_f32x2(add_f32x2(sum[0], sum[1]));
                 l += add.x + add.y;
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(p_full + s);
+                mbar_arrive(p_full + 2 * s + buf);
             }
-            bool ok = mbar_wait(o_full + s, mine++ & 1, abort_flag, p.err, kErrAccWait);
+            loads += 2 * tiles;
+            bool ok = mbar_wait(o_done + 2 * s + 1, mine++ & 1, abort_flag, p.err, kErrAccWait);
             if (!__all_sync(0xffffffffu, ok)) return false;
             tc_fence_after();
             const size_t at = (size_t)slot * p.batch.rows * p.q_heads + unit;
