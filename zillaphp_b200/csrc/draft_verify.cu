@@ -6,9 +6,13 @@
 //   accept d_j while u_j q_j(d_j) < p_j(d_j); a = the number accepted;
 //   w = max(p_a - q_a, 0) where a draft failed, p_a behind the last one;
 //   the token drawn is the lowest t with w_0 + ... + w_t > r (w_0 + ... + w_{V-1}), r = u_k.
-// Differences, sums and the product are fp64: fp32 sums over a large vocabulary are off by more than
-// the distance between neighbouring borders, and would make the token depend on how a row is split.
+// fp32 sums over a large vocabulary are off by more than the distance between neighbouring borders, and would make
+// the token depend on how a row is split: differences are exact and sums are kept to 46 bits or more, a warp's
+// part of a row as pairs of fp32 numbers, everything else in fp64.
 #include <cooperative_groups.h>
+#include <float.h>
+
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
@@ -17,7 +21,7 @@ namespace cg = cooperative_groups;
 namespace zb {
 namespace {
 
-constexpr int kVerifyThreads = 512;
+constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyMaxCluster = 8;
 
@@ -32,16 +36,34 @@ struct VerifyParams {
 };
 
 // w_t of one element in fp64; NaN counts as 0.
-__device__ __forceinline__ double residual(float p, float q) { return fmax((double)p - (double)q, 0.0); }
+__device__ __forceinline__ double residual(float p, float q) { return p > q ? (double)fminf(p, FLT_MAX) - (double)q : 0.0; }
+
+// The sum of many residuals as an unevaluated sum hi + lo of fp32 numbers: the difference p - q = d + e is exact
+// (Dekker 1971, p > q >= 0; a negative q costs at most lo's rounding), hi + d = h + t too (Knuth's two-sum), and lo
+// takes e and t.  Eleven additions on the fp32 pipe; the same sum in fp64 is bound by two conversions an element (47 us
+// against 29 us for 192 rows of 100,003).
+struct PairSum {
+    float hi = 0.0f, lo = 0.0f;
+    __device__ __forceinline__ void add(float p, float q, bool keep) {
+        if (!(p > q) || !keep) p = q = 0.0f;
+        p = fminf(p, FLT_MAX);
+        const float d = p - q, e = (p - d) - q;
+        const float h = hi + d, b = h - hi, t = (hi - (h - b)) + (d - b);
+        hi = h;
+        lo += e + t;
+    }
+};
 
 // Bound by HBM: one row of p, and one of q where a draft failed, read once by the sequence's cluster.
 // Each warp sums one segment of the row; the segments' sums meet in the cluster's shared memory, and the
 // block that owns the crossing segment reads it again (it is in L2) to find the token.
+// Six blocks an SM (40 registers a thread), so that blocks that look for their row or for their token leave enough others
+// that stream: 29 us against 36 with four.
 template <bool VEC>
-__global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const VerifyParams a) {
+__global__ void __launch_bounds__(kVerifyThreads, 6) draft_verify_kernel(const VerifyParams a) {
     __shared__ double sums[kVerifyWarps];                      // read by the whole cluster
     __shared__ double all[kVerifyMaxCluster * kVerifyWarps];
-    __shared__ double part[kVerifyWarps], s_base, s_target, s_total;
+    __shared__ double part[kVerifyWarps], s_base, s_target;
     __shared__ int s_taken, s_seg, s_found, s_last;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -95,35 +117,67 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
         auto w = [&](int i) { return i == skip ? 0.0 : residual(p[i], q ? q[i] : 0.0f); };
         const long long lo = (long long)(rank * kVerifyWarps + warp) * a.seg;
         const int begin = (int)min(lo, (long long)V), end = (int)min(lo + a.seg, (long long)V);
-        double s = 0.0;
-        if constexpr (VEC) {
-            int i = begin + 4 * lane;
-#pragma unroll 4
-            for (; i + 3 < end; i += 128) {
-                const float4 x = *reinterpret_cast<const float4 *>(p + i);
-                const float4 y = q ? *reinterpret_cast<const float4 *>(q + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                double e[4] = {residual(x.x, y.x), residual(x.y, y.y), residual(x.z, y.z), residual(x.w, y.w)};
+        PairSum sum;
+        auto take = [&](int i, float x, float y) { sum.add(x, y, i != skip); };
+        // a batch of loads in front of its sums: 64 bytes a thread in flight
+        auto stream = [&](auto with_q) {
+            constexpr bool kQ = decltype(with_q)::value;
+            if constexpr (VEC) {
+                constexpr int kBatch = kQ ? 2 : 4;
+                auto part4 = [&](int i, const float4 &x, const float4 &y) {
+                    take(i, x.x, y.x);
+                    take(i + 1, x.y, y.y);
+                    take(i + 2, x.z, y.z);
+                    take(i + 3, x.w, y.w);
+                };
+                int i = begin + 4 * lane;
+                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (; i + 3 + 128 * (kBatch - 1) < end; i += 128 * kBatch) {
+                    float4 x[kBatch], y[kBatch];
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    if (i + t == skip) e[t] = 0.0;
-                s += (e[0] + e[1]) + (e[2] + e[3]);
+                    for (int e = 0; e < kBatch; ++e) {
+                        x[e] = *reinterpret_cast<const float4 *>(p + i + 128 * e);
+                        y[e] = kQ ? *reinterpret_cast<const float4 *>(q + i + 128 * e) : zero;
+                    }
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) part4(i + 128 * e, x[e], y[e]);
+                }
+                for (; i + 3 < end; i += 128)
+                    part4(i, *reinterpret_cast<const float4 *>(p + i), kQ ? *reinterpret_cast<const float4 *>(q + i) : zero);
+                for (; i < end; ++i) take(i, p[i], kQ ? q[i] : 0.0f);   // the row's last one to three elements, one lane's
+            } else {
+                constexpr int kBatch = kQ ? 4 : 8;
+                int i = begin + lane;
+                for (; i + 32 * (kBatch - 1) < end; i += 32 * kBatch) {
+                    float x[kBatch], y[kBatch];
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) {
+                        x[e] = p[i + 32 * e];
+                        y[e] = kQ ? q[i + 32 * e] : 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) take(i + 32 * e, x[e], y[e]);
+                }
+                for (; i < end; i += 32) take(i, p[i], kQ ? q[i] : 0.0f);
             }
-            for (; i < end; ++i) s += w(i);   // the row's last one to three elements, one lane's
-        } else {
-#pragma unroll 8
-            for (int i = begin + lane; i < end; i += 32) s += w(i);
-        }
+        };
+        if (q) stream(std::true_type());
+        else stream(std::false_type());
+        double s = (double)sum.hi + (double)sum.lo;
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) sums[warp] = s;
         cluster.sync();
         for (int i = tid; i < kVerifyMaxCluster * kVerifyWarps; i += kVerifyThreads)
             all[i] = i < ranks * kVerifyWarps ? cluster.map_shared_rank(sums, i / kVerifyWarps)[i % kVerifyWarps] : 0.0;
-        cluster.sync();   // no block leaves, or sums again, while another still reads
-        if (warp == 0) {  // four segments a lane; every block works out the same
-            static_assert(kVerifyMaxCluster * kVerifyWarps == 128, "four segments a lane");
-            const double *v = all + 4 * lane;
-            double incl = (v[0] + v[1]) + (v[2] + v[3]);
+        cluster.barrier_arrive();   // waited for below: no block leaves, or sums again, while another still reads
+        __syncthreads();
+        if (warp == 0) {  // every block works out the same
+            constexpr int kEach = kVerifyMaxCluster * kVerifyWarps / 32;   // segments a lane
+            const double *v = all + kEach * lane;
+            double incl = 0.0;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) incl += v[e];
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double up = __shfl_up_sync(0xffffffffu, incl, o);
@@ -135,9 +189,9 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
             int hit = -1, last = -1;
             double hit_base = 0.0, last_base = 0.0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < kEach; ++e) {
                 if (v[e] > 0.0) {
-                    last = 4 * lane + e;
+                    last = kEach * lane + e;
                     last_base = run;
                     if (hit < 0 && run + v[e] > target) {
                         hit = last;
@@ -153,7 +207,6 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
                 s_seg = hits ? hit : last;   // -1: nothing to draw from
                 s_base = hits ? hit_base : last_base;
                 s_target = target;
-                s_total = total;
             }
         }
         if (tid == 0) {
@@ -161,18 +214,16 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
             s_last = -1;
         }
         __syncthreads();
-        if (s_seg >= 0 || pass == 1) {
-            const int seg = s_seg;
-            if (seg < 0) {
-                if (rank == 0 && tid == 0) a.tokens[row] = 0;
-                return;
-            }
-            if (seg / kVerifyWarps != rank) return;
+        const int seg = s_seg;
+        if (seg < 0 && pass == 1) {
+            if (rank == 0 && tid == 0) a.tokens[row] = 0;
+        } else if (seg >= 0 && seg / kVerifyWarps == rank) {
             // the whole block reads the crossing segment again: a few neighbours a thread
             const long long from = (long long)seg * a.seg;
             const int stop = (int)min(from + a.seg, (long long)V), per = (a.seg + kVerifyThreads - 1) / kVerifyThreads;
             const int i0 = min((int)from + tid * per, stop), i1 = min(i0 + per, stop);
             double mine = 0.0;
+#pragma unroll 8
             for (int i = i0; i < i1; ++i) mine += w(i);
             double incl = mine;
 #pragma unroll
@@ -198,8 +249,9 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
             if (last >= 0) atomicMax(&s_last, last);
             __syncthreads();
             if (tid == 0) a.tokens[row] = s_found != 0x7fffffff ? s_found : s_last;
-            return;
         }
+        cluster.barrier_wait();
+        if (seg >= 0) return;
         q = nullptr;
         skip = -1;
         __syncthreads();   // s_seg is read by all before it is written again
@@ -246,10 +298,10 @@ extern "C" int draft_verify_dev(int p_id, int p_ld, int q_id, int q_ld, int draf
     a.vocab = vocab;
     a.err = device_error_word();
     if (!a.err) return fail(kBadHandle, "%s: no device error word", name);
-    // blocks to a sequence: doubled while the batch leaves SMs without two blocks and a block would
-    // still have 4096 elements, eight for each of its threads
+    // blocks to a sequence: as many as leave a block 4096 elements, up to eight; fewer where that would be more than
+    // four rounds over the machine (six blocks an SM), since each block first finds its row
     int ranks = 1;
-    while (ranks < kVerifyMaxCluster && (long long)batch * ranks < 2 * sm_count() && vocab / (2 * ranks) >= 4096) ranks *= 2;
+    while (ranks < kVerifyMaxCluster && vocab / (ranks + 1) >= 4096 && (long long)batch * (ranks + 1) <= 24LL * sm_count()) ++ranks;
     const int warps = ranks * kVerifyWarps;
     a.seg = ((vocab + warps - 1) / warps + 127) / 128 * 128;
     if ((long long)batch * ranks > 0x7fffffffLL) return fail(kBadArg, "%s: batch %d is too large", name, batch);
@@ -267,8 +319,7 @@ extern "C" int draft_verify_dev(int p_id, int p_ld, int q_id, int q_ld, int draf
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    if (vec) cudaLaunchKernelEx(&cfg, draft_verify_kernel<true>, a);
-    else cudaLaunchKernelEx(&cfg, draft_verify_kernel<false>, a);
+    cudaLaunchKernelEx(&cfg, vec ? draft_verify_kernel<true> : draft_verify_kernel<false>, a);
     ZB_LAUNCH_CHECK(name);
     return kOk;
 }
