@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
         int it = 0;
         for (; it < steps; ++it) {
             const int st = it % ST, at = lane < all ? box_row(p, pages, head, begin + it * kTile + r0, end) : 0;
-            ok = it < ST || mbar_wait(empty + st, (it / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
+            ok = it < ST || wait_phase(empty + st, (it / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(full + st, 2 * kTileBytes);
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
     bool ok = true;
     for (int it = 0; it < steps; ++it) {
         const int st = it % ST, key0 = begin + it * kTile + wn * KW;
-        ok = mbar_wait(full + st, (it / ST) & 1, abort_flag, p.err, kErrFullWait);
+        ok = wait_phase(full + st, (it / ST) & 1, abort_flag, p.err, kErrFullWait);
         if (!__all_sync(0xffffffffu, ok)) break;
         const uint32_t sk = smem_u32(base) + 2 * st * kTileBytes, sv = sk + kTileBytes;
         float s[NT][4];

@@ -81,6 +81,24 @@ __device__ __forceinline__ int box_row(const AttendParams &p, const int *pages, 
     return ((id * p.kv_heads + kv_head) << p.page_log2) + (key & ((1 << p.page_log2) - 1));
 }
 
+// tc::mbar_wait with the clock read only after 64 failed tries: reading %globaltimer between the first two tries delays
+// nearly every wait of these kernels' handshakes by that read.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort, int *err, int code) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; ++i) {
+        if (tc::mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 0u) {
+            if (*abort) return false;
+            const uint64_t t = tc::global_ns();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > tc::kWaitLimitNs) break;
+        }
+    }
+    *abort = 1;
+    if (err) atomicCAS(err, 0, code);
+    return false;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

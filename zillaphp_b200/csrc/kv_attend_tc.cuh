@@ -14,7 +14,8 @@
 // ref is the row's maximum as of its last change: it follows the true maximum only when that has passed it
 // by 2^8 (then O and l are rescaled), so that O rarely has to travel through registers; weights stay
 // below 2^8 and l and O carry the same factor, so the quotient does not change.
-// Warps 0-3 and 4-7 are the streams' softmax, warp 8 loads (TMA through the page list), warp 9 issues the MMAs.
+// Warps 0-3 and 4-7 are the streams' softmax, warp 8 loads (TMA through the page list), warps 9 and 10 issue the streams'
+// MMAs (one warp for both waits for one stream's softmax while the other's step could run: PLACEHOLDER).
 //
 // Order of a stream's MMAs: P V of step h, then Q K^T of step h + 2 over the same TMEM columns; one thread
 // issues both and the tensor pipe takes them in order.
@@ -29,7 +30,7 @@ using namespace tc;
 
 constexpr int kTcTile = 128;      // rows of a stream, keys of a tile
 constexpr int kTcStep = 64;       // keys of a step
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 352;
 
 template <int D>
 constexpr int tc_stages() { return D == 128 ? 5 : 8; }
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
     uint8_t *ring = base + 2 * kTileBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + ST * kTileBytes);
     uint64_t *full = bars, *empty = bars + ST, *q_full = bars + 2 * ST, *s_full = q_full + 1, *p_full = s_full + 4, *o_done = p_full + 4, *drain = o_done + 4;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -139,15 +140,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(full + i, 1);
-            mbar_init(empty + i, 1);
+            mbar_init(empty + i, 2);        // both streams
         }
-        mbar_init(q_full, 2 * kTcTile);
+        mbar_init(q_full, 8);
         for (int i = 0; i < 4; ++i) {   // [stream][step & 1]: a waiter is at most one phase behind
             mbar_init(s_full + i, 1);
-            mbar_init(p_full + i, kTcTile);
+            mbar_init(p_full + i, 4);       // one arrival a warp: 128 on one barrier queue up behind each other
             mbar_init(o_done + i, 1);
         }
         mbar_init(drain, 1);
+        mbar_init(drain + 1, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             for (int x = 0; x < 2 * tiles; ++x, ++i) {
                 const int st = i % ST;
                 const int at = lane < all ? box_row(p, p.prefix_pages, head, (tile0 + (x >> 1)) * kTcTile + r0, p.batch.prefix_len) : 0;
-                ok = i < ST || mbar_wait(empty + st, (i / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
+                ok = i < ST || wait_phase(empty + st, (i / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) return false;
                 if (lane == 0) mbar_arrive_expect_tx(full + st, kTileBytes);
@@ -182,9 +184,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         if (!ok && lane == 0)   // the copies in flight end before the block's shared memory goes
             for (int x = max(0, i - ST); x < i; ++x)
                 if (!mbar_wait_drain(full + x % ST, (x / ST) & 1)) atomicCAS(p.err, 0, kErrDrain);
-    } else if (warp == 9) {
-        // ---- MMAs.  The whole warp runs the loop, one elected lane issues: addresses stay in uniform registers, and a
-        // step's twelve MMAs follow each other without work between them.
+    } else if (warp > 8) {
+        // ---- MMAs of one stream.  The whole warp runs the loop, one elected lane issues: addresses stay in uniform
+        // registers, and a step's twelve MMAs follow each other without work between them.
+        const int s = warp - 9;
         constexpr uint32_t kIdS = attend_idesc<T>(kTcStep, false), kIdO = attend_idesc<T>(D, true);
         constexpr uint32_t kStep16 = kTcStep * kRowBytes / 16, kTile16 = kTileBytes / 16;   // in the descriptors' units of 16 bytes
         const uint64_t q_desc = smem_desc(smem_u32(base), 16, kAtom, kSw), k_desc = smem_desc(smem_u32(ring), 16, kAtom, kSw),
@@ -198,27 +201,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                 }
             }
         };
-        auto wait_load = [&](const Place &x) { return mbar_wait(full + x.st, x.turn, abort_flag, p.err, kErrFullWait); };
-        auto qk = [&](int s, int h, int st) {   // step h of the segment, whose K is in stage st
-            const uint64_t a = q_desc + s * kTile16, b = k_desc + st * kTile16 + (h & 1) * kStep16;
-            const uint32_t d = tmem + s * 128 + (h & 1) * kTcStep;
+        auto wait_load = [&](const Place &x) { return wait_phase(full + x.st, x.turn, abort_flag, p.err, kErrFullWait); };
+        const uint32_t s_at = tmem + s * 128, o_at = tmem + 256 + s * D;
+        auto qk = [&](int h, int st) {   // step h of a tile, whose K is in stage st
+            const uint64_t a = q_desc + s * kTile16, b = k_desc + st * kTile16 + h * kStep16;
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t at = ((k >> 2) * kHalfBytes + (k & 3) * 32) / 16;
-                    mma_bf16(d, a + at, b + at, kIdS, k != 0);
+                    mma_bf16(s_at + h * kTcStep, a + at, b + at, kIdS, k != 0);
                 }
-                mma_commit(s_full + 2 * s + (h & 1));
+                mma_commit(s_full + 2 * s + h);
             }
             __syncwarp();
         };
-        auto pv = [&](int s, int h, int st, bool last) {
-            const uint64_t b = v_desc + st * kTile16 + (h & 1) * kStep16;
-            const uint32_t a = tmem + s * 128 + (h & 1) * kTcStep, d = tmem + 256 + s * D;
+        auto pv = [&](int h, int st, bool more, bool last) {
+            const uint64_t b = v_desc + st * kTile16 + h * kStep16;
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kTcStep / 16; ++k) mma_f16_ta(d, a + 8 * k, b + k * (2 * kAtom / 16), kIdO, h > 0 || k != 0);
-                if (last) mma_commit(o_done + 2 * s + (h & 1));
+                for (int k = 0; k < kTcStep / 16; ++k)
+                    mma_f16_ta(o_at, s_at + h * kTcStep + 8 * k, b + k * (2 * kAtom / 16), kIdO, more || k != 0);
+                if (last) mma_commit(o_done + 2 * s + h);
             }
             __syncwarp();
         };
@@ -227,41 +230,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             __syncwarp();
         };
         bool ok = true;
-        int done[2] = {0, 0}, segment = 0;   // pairs of steps of each stream, segments
-        Place k_at, v_at;                    // the tile's K and V
+        int done = 0, segment = 0;   // tiles of this stream, segments
+        Place k_at, v_at;            // the tile's K and V
         v_at.next();
         segments([&](int, int, int streams, int, int tiles, int) {
-            ok = mbar_wait(q_full, segment++ & 1, abort_flag, p.err, kErrFullWait) && wait_load(k_at);
+            if (s >= streams) {      // no rows: the tiles are handed back
+                ok = wait_phase(q_full, segment++ & 1, abort_flag, p.err, kErrFullWait);   // not to be two phases ahead of it later
+                if (!ok) return false;
+                for (int x = 0; x < 2 * tiles; ++x) {
+                    Place &at = x & 1 ? v_at : k_at;
+                    ok = wait_load(at);
+                    if (!ok) return false;
+                    if (lane == 0) mbar_arrive(empty + at.st);
+                    at.next();
+                    at.next();
+                }
+                return true;
+            }
+            ok = wait_phase(q_full, segment++ & 1, abort_flag, p.err, kErrFullWait) && wait_load(k_at);
             if (!ok) return false;
             tc_fence_after();
-            for (int h = 0; h < 2; ++h)
-                for (int s = 0; s < streams; ++s) qk(s, h, k_at.st);
+            qk(0, k_at.st);
+            qk(1, k_at.st);
             release(k_at.st);
-            for (int j = 0; j < tiles; ++j) {
+            for (int j = 0; j < tiles; ++j, ++done) {
                 const bool more = j + 1 < tiles;
                 k_at.next();
                 k_at.next();
-                ok = wait_load(v_at);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    for (int s = 0; ok && s < streams; ++s) {
-                        ok = mbar_wait(p_full + 2 * s + h, done[s] & 1, abort_flag, p.err, kErrAccWait);
-                        if (!ok) break;
-                        tc_fence_after();
-                        pv(s, 2 * j + h, v_at.st, !more);
-                        if (more) {
-                            if (h == 0 && s == 0) {
-                                ok = wait_load(k_at);
-                                if (!ok) break;
-                                tc_fence_after();
-                            }
-                            qk(s, h, k_at.st);
-                        }
-                        done[s] += h;
-                    }
+                ok = wait_load(v_at) && (!more || wait_load(k_at)) && wait_phase(p_full + 2 * s, done & 1, abort_flag, p.err, kErrAccWait);
                 if (!ok) return false;
+                tc_fence_after();
+                pv(0, v_at.st, j > 0, !more);
+                if (more) qk(0, k_at.st);
+                ok = wait_phase(p_full + 2 * s + 1, done & 1, abort_flag, p.err, kErrAccWait);
+                if (!ok) return false;
+                tc_fence_after();
+                pv(1, v_at.st, true, !more);
                 release(v_at.st);
-                if (more) release(k_at.st);
+                if (more) {
+                    qk(1, k_at.st);
+                    release(k_at.st);
+                }
                 v_at.next();
                 v_at.next();
             }
@@ -269,8 +278,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         });
         if (!ok) {   // MMAs in flight end before TMEM goes
             if (elect_one()) {
-                mma_commit(drain);
-                if (!mbar_wait_drain(drain, 0)) atomicCAS(p.err, 0, kErrDrain);
+                mma_commit(drain + s);
+                if (!mbar_wait_drain(drain + s, 0)) atomicCAS(p.err, 0, kErrDrain);
             }
             __syncwarp();
         }
@@ -283,9 +292,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         int done = 0, loads = 0, segment = 0, mine = 0;   // steps of this stream, loads of the ring, segments, this stream's segments
         segments([&](int head, int row0, int streams, int tile0, int tiles, int slot) {
             if (s >= streams) {   // no rows here; not to arrive for the next segment before this one's queries are there
-                mbar_arrive(q_full);
+                if (lane == 0) mbar_arrive(q_full);
                 loads += 2 * tiles;
-                return __all_sync(0xffffffffu, mbar_wait(q_full, segment++ & 1, abort_flag, p.err, kErrAccWait)) != 0;
+                return __all_sync(0xffffffffu, wait_phase(q_full, segment++ & 1, abort_flag, p.err, kErrAccWait)) != 0;
             }
             ++segment;
             const int row = row0 + s * kTcTile + r;
@@ -303,12 +312,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                     *reinterpret_cast<uint4 *>(base + s * kTileBytes + tile_chunk<D>(r, c, kTcTile)) = x;
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(q_full);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
             }
             float ref = 0.0f, l = 0.0f;   // ref in units of log2
             for (int h = 0; h < 2 * tiles; ++h, ++done) {
                 const int buf = h & 1;
-                bool ok = mbar_wait(s_full + 2 * s + buf, (done >> 1) & 1, abort_flag, p.err, kErrAccWait);
+                bool ok = wait_phase(s_full + 2 * s + buf, (done >> 1) & 1, abort_flag, p.err, kErrAccWait);
                 if (!__all_sync(0xffffffffu, ok)) return false;
                 tc_fence_after();
                 uint32_t v[2][32];
@@ -327,7 +337,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                     }
                     if (!buf) {   // V behind the last key counts as zero, whatever its page holds
                         const int load = loads + h + 1, st = load % ST;
-                        ok = mbar_wait(full + st, (load / ST) & 1, abort_flag, p.err, kErrFullWait);
+                        ok = wait_phase(full + st, (load / ST) & 1, abort_flag, p.err, kErrFullWait);
                         if (!__all_sync(0xffffffffu, ok)) return false;
                         for (int x = r; x < (kTcTile - left) * (D / 8); x += kTcTile)
                             *reinterpret_cast<uint4 *>(ring + st * kTileBytes + tile_chunk<D>(left + x / (D / 8), x % (D / 8), kTcTile)) =
@@ -347,8 +357,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                 if (h == 0) ref = m;
                 else if (__any_sync(0xffffffffu, m > ref + 8.0f)) {
                     // O with the step before in it: S of the next step is committed behind that, or the segment's last steps themselves
-                    ok = h + 1 < 2 * tiles ? mbar_wait(s_full + 2 * s + (buf ^ 1), ((done + 1) >> 1) & 1, abort_flag, p.err, kErrAccWait)
-                                           : mbar_wait(o_done + 2 * s + (buf ^ 1), mine & 1, abort_flag, p.err, kErrAccWait);
+                    ok = h + 1 < 2 * tiles ? wait_phase(s_full + 2 * s + (buf ^ 1), ((done + 1) >> 1) & 1, abort_flag, p.err, kErrAccWait)
+                                           : wait_phase(o_done + 2 * s + (buf ^ 1), mine & 1, abort_flag, p.err, kErrAccWait);
                     if (!__all_sync(0xffffffffu, ok)) return false;
                     tc_fence_after();
                     const float f = m > ref ? ex2(ref - m) : 1.0f;
@@ -384,10 +394,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
                 l += add.x + add.y;
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(p_full + 2 * s + buf);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 2 * s + buf);
             }
             loads += 2 * tiles;
-            bool ok = mbar_wait(o_done + 2 * s + 1, mine++ & 1, abort_flag, p.err, kErrAccWait);
+            bool ok = wait_phase(o_done + 2 * s + 1, mine++ & 1, abort_flag, p.err, kErrAccWait);
             if (!__all_sync(0xffffffffu, ok)) return false;
             tc_fence_after();
             const size_t at = (size_t)slot * p.batch.rows * p.q_heads + unit;
