@@ -272,52 +272,71 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
     }
 }
 
-// The join: one warp a (row, query head), each lane D / 32 columns.  Reads the slots' parts once, mostly
-// from L2; a row of no sequence is left as it is, a row without keys becomes zero.
+// The join: one warp a (row, query head), each lane D / 32 columns.  Reads the slots' parts once, mostly from L2, eight
+// slots at a time (their addresses do not depend on their maxima, so all loads of a row are on the way together); a row
+// of no sequence is left as it is, a row without keys becomes zero.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p) {
-    constexpr int C = D / 32;
-    __shared__ int owner[9];
+    constexpr int C = D / 32, kBatch = 8;
+    __shared__ int owner[8], own_slots[8];   // of the block's tokens, eight at most
     griddep_launch();
+    const int tid = threadIdx.x, lane = tid & 31;
+    const long long unit0 = (long long)blockIdx.x * 8, units = (long long)p.batch.rows * p.q_heads, unit = unit0 + (tid >> 5);
+    const int t0 = (int)(unit0 / p.q_heads), n = (int)(min(unit0 + 8, units) - 1) / p.q_heads - t0 + 1;
+    const int t = (int)(unit / p.q_heads), hq = (int)(unit - (long long)t * p.q_heads);
+    if (tid < 8) owner[tid] = -1;
     griddep_wait();
-    const long long unit0 = (long long)blockIdx.x * 8, units = (long long)p.batch.rows * p.q_heads;
-    const int t0 = (int)(unit0 / p.q_heads), t1 = (int)(min(unit0 + 8, units) - 1) / p.q_heads;
-    kv_owners(owner, p.batch.start, p.batch.batch, t0, t1 - t0 + 1, threadIdx.x, 256);
-    const int lane = threadIdx.x & 31;
-    const long long unit = unit0 + (threadIdx.x >> 5);
-    if (unit >= units) return;
-    const int t = (int)(unit / p.q_heads), b = owner[t - t0];
-    if (b < 0) return;
-    int first, n, len;
-    load_sequence(p, b, first, n, len);
-    if (n == 0) return;
-    const int own = (min(len, own_limit(len, n, t - first)) + p.own_chunk - 1) / p.own_chunk;
     int front = p.prefix_splits;   // the prefix's slots come first
-    if (p.tc_blocks) {
-        const int hq = (int)(unit - (long long)t * p.q_heads), row = t * p.group + hq % p.group;
-        front = prefix_cut(p.batch.prefix_len, p.kv_heads * p.prefix_tiles, p.tc_blocks).slots(hq / p.group * p.prefix_tiles + row / (2 * kTcTile));
+    if (p.tc_blocks && unit < units) {
+        const int head = hq / p.group, row = t * p.group + hq - head * p.group;
+        front = p.item_slots[head * p.prefix_tiles + row / (2 * kTcTile)];
     }
-    const int slots = front + own, skip = p.prefix_splits - front;   // the own ones lie behind the most that the prefix can have
-    float m = -INFINITY;
-    for (int s = lane; s < slots; s += 32) m = fmaxf(m, p.part_ml[(s < front ? s : s + skip) * units + unit].x);
+    __syncthreads();
+    for (int b = tid; b < p.batch.batch; b += 256) {   // every sequence looked at by one thread: no chain of dependent loads
+        const int first = p.batch.start[b], next = p.batch.start[b + 1], len = p.batch.len[b];
+        const int lo = max(first, t0), hi = min(next, t0 + n);
+        if (lo < hi && sequence_fits(p, first, next - first, len))
+            for (int x = lo; x < hi; ++x) {
+                owner[x - t0] = b;
+                own_slots[x - t0] = (min(len, own_limit(len, next - first, x - first)) + p.own_chunk - 1) / p.own_chunk;
+            }
+    }
+    __syncthreads();
+    if (unit >= units || owner[t - t0] < 0) return;
+    const int slots = front + own_slots[t - t0], skip = p.prefix_splits - front;   // the own ones lie behind the most that the prefix can have
+    float m = -INFINITY, acc[C] = {}, l = 0.0f;
+    for (int s0 = 0; s0 < slots; s0 += kBatch) {
+        float2 ml[kBatch];
+        float v[kBatch][C];
 #pragma unroll
-    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    if (m == -INFINITY) m = 0.0f;
-    float acc[C] = {}, l = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < slots; ++s) {
-        const long long at = (s < front ? s : s + skip) * units + unit;
-        const float2 ml = p.part_ml[at];
-        const float w = ex2(ml.x - m);
-        float v[C];
-        load_vec<float, C>(p.part_o + at * D + lane * C, v);
-        l += w * ml.y;
+        for (int i = 0; i < kBatch; ++i) {
+            const int s = s0 + i;
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            if (s >= slots) continue;
+            const long long at = (s < front ? s : s + skip) * units + unit;
+            ml[i] = p.part_ml[at];
+            load_vec<float, C>(p.part_o + at * D + lane * C, v[i]);
+        }
+        float top = m;
 #pragma unroll
-        for (int i = 0; i < C; ++i) acc[i] += w * v[i];
+        for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
+        const float use = top == -INFINITY ? 0.0f : top, f = ex2(m - use);
+        m = top;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (s0 + i >= slots) continue;
+            const float w = ex2(ml[i].x - use);
+            l += w * ml[i].y;
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] += w * v[i][c];
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < C; ++i) acc[i] *= inv;
+    for (int c = 0; c < C; ++c) acc[c] *= inv;
     store_vec<T, C>(static_cast<T *>(p.out) + unit * D + lane * C, acc);
 }
 
@@ -387,6 +406,7 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
     p.direct = p.own_splits == 1 && p.prefix_splits == 0;
     p.units = (size_t)rows * q_heads;
     p.part_floats = p.direct ? 0 : p.units * (p.own_splits + p.prefix_splits) * (c.head_dim + 2);
+    if (p.tc_blocks) p.part_floats += (size_t)c.kv_heads * p.prefix_tiles;   // the items' slots
     return p;
 }
 
@@ -502,6 +522,8 @@ int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int 
             return rc;
     if (plan.part_floats)
         if (int rc = check_buffers(name, {{work_id, plan.part_floats, "work"}})) return rc;
+    if ((long long)plan.prefix_tiles * c->kv_heads * (prefix_len / kTcTile + 1) > 0x7fffffffLL)
+        return fail(kBadArg, "%s: prefix of %d tokens for %d rows is too large", name, prefix_len, rows);
     if (!batch || !rows) return kOk;
     AttendParams p;
     p.k_map = c->k_map;
@@ -511,6 +533,7 @@ int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int 
     p.part_o = plan.part_floats ? ptr(work_id) : nullptr;
     const size_t slots = (size_t)plan.own_splits + plan.prefix_splits;
     p.part_ml = plan.part_floats ? reinterpret_cast<float2 *>(ptr(work_id) + plan.units * slots * c->head_dim) : nullptr;
+    p.item_slots = plan.part_floats ? reinterpret_cast<int *>(ptr(work_id) + plan.units * slots * (c->head_dim + 2)) : nullptr;
     p.batch = {reinterpret_cast<const int *>(ptr(start_id)), reinterpret_cast<const int *>(ptr(len_id)),
                reinterpret_cast<const int *>(ptr(pages_id)), batch, rows, max_pages, prefix_len};
     p.prefix_pages = prefix_len ? reinterpret_cast<const int *>(ptr(prefix_pages_id)) : nullptr;

@@ -20,6 +20,7 @@ struct AttendParams {
     void *out;
     float *part_o;      // [slots][rows * q_heads][head_dim]
     float2 *part_ml;    // [slots][rows * q_heads]
+    int *item_slots;    // the tcgen05 kernel's items: how many slots each took
     KvBatch batch;
     const int *prefix_pages;
     int q_heads, kv_heads, group, page_log2, pages, box_rows;
@@ -38,17 +39,14 @@ struct AttendParams {
 // item; block c of n takes units [c U / n, (c + 1) U / n), so that no block has more than a tile over another, whatever the
 // counts.  An item's slots are the blocks that touch it, in order.
 struct PrefixCut {
-    long long units;
-    int tiles, blocks;
-    __host__ __device__ long long begin(int c) const { return c * units / blocks; }
-    __host__ __device__ int block_of(long long unit) const { return (int)(((unit + 1) * blocks - 1) / units); }
-    __host__ __device__ int first_block(int item) const { return block_of((long long)item * tiles); }
-    __host__ __device__ int slots(int item) const { return block_of((long long)(item + 1) * tiles - 1) - first_block(item) + 1; }
+    int units, tiles, blocks;   // units * blocks may pass 31 bits
+    __host__ __device__ int begin(int c) const { return (int)((long long)c * units / blocks); }
+    __host__ __device__ int first_block(int item) const { return (int)((((long long)item * tiles + 1) * blocks - 1) / units); }
 };
 __host__ __device__ __forceinline__ PrefixCut prefix_cut(int prefix_len, int items, int blocks) {
     PrefixCut c;
     c.tiles = (prefix_len + 127) / 128;
-    c.units = (long long)items * c.tiles;
+    c.units = items * c.tiles;
     c.blocks = blocks;
     return c;
 }
@@ -56,12 +54,16 @@ __host__ __device__ __forceinline__ PrefixCut prefix_cut(int prefix_len, int ite
 // Keys that row j of a sequence sees of its own: clamped to 0 .. len.
 __device__ __forceinline__ int own_limit(int len, int n, int j) { return max(0, len - n + j + 1); }
 
+__device__ __forceinline__ bool sequence_fits(const AttendParams &p, int first, int n, int len) {
+    return first >= 0 && n >= 0 && n <= p.max_new && (long long)first + n <= p.batch.rows && len >= 0 && len <= p.max_len;
+}
+
 // A sequence's new rows and length; one that does not fit the call's sizes is recorded and has no rows.
 __device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int &first, int &n, int &len) {
     first = __ldcg(p.batch.start + b);
     n = __ldcg(p.batch.start + b + 1) - first;
     len = __ldcg(p.batch.len + b);
-    if (first < 0 || n < 0 || n > p.max_new || (long long)first + n > p.batch.rows || len < 0 || len > p.max_len) {
+    if (!sequence_fits(p, first, n, len)) {
         atomicCAS(p.err, 0, kErrKvLength);
         n = 0;
         len = 0;

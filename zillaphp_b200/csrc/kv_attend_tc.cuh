@@ -126,13 +126,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
 
     const int rows = p.batch.rows * p.group;
     const PrefixCut cut = prefix_cut(p.batch.prefix_len, p.kv_heads * p.prefix_tiles, p.tc_blocks);
-    const long long unit0 = cut.begin(blockIdx.x), unit1 = cut.begin(blockIdx.x + 1);
-    // the block's segments in order, the same in every role: fn(kv head, first row, streams, first tile, tiles, slot) until it returns false
+    const int unit0 = cut.begin(blockIdx.x), unit1 = cut.begin(blockIdx.x + 1);
+    // the block's segments in order, the same in every role: fn(item, first row, streams, first tile, tiles) until it returns false
     auto segments = [&](auto fn) {
-        for (long long unit = unit0; unit < unit1;) {
-            const int item = (int)(unit / cut.tiles), tile0 = (int)(unit - (long long)item * cut.tiles);
-            const int tiles = (int)min((long long)(cut.tiles - tile0), unit1 - unit), row0 = item % p.prefix_tiles * 2 * kTcTile;
-            if (!fn(item / p.prefix_tiles, row0, rows - row0 > kTcTile ? 2 : 1, tile0, tiles, (int)blockIdx.x - cut.first_block(item))) return;
+        for (int unit = unit0; unit < unit1;) {
+            const int item = unit / cut.tiles, tile0 = unit - item * cut.tiles, tiles = min(cut.tiles - tile0, unit1 - unit);
+            const int row0 = item % p.prefix_tiles * 2 * kTcTile;
+            if (!fn(item, row0, rows - row0 > kTcTile ? 2 : 1, tile0, tiles)) return;
             unit += tiles;
         }
     };
@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         const int r0 = lane % boxes * p.box_rows, half = lane / boxes;
         bool ok = true;
         int i = 0;   // loads so far: K of a tile, then V
-        segments([&](int head, int, int, int tile0, int tiles, int) {
+        segments([&](int item, int, int, int tile0, int tiles) {
+            const int head = item / p.prefix_tiles;
             for (int x = 0; x < 2 * tiles; ++x, ++i) {
                 const int st = i % ST;
                 const int at = lane < all ? box_row(p, p.prefix_pages, head, (tile0 + (x >> 1)) * kTcTile + r0, p.batch.prefix_len) : 0;
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         int done = 0, segment = 0;   // tiles of this stream, segments
         Place k_at, v_at;            // the tile's K and V
         v_at.next();
-        segments([&](int, int, int streams, int, int tiles, int) {
+        segments([&](int, int, int streams, int, int tiles) {
             if (s >= streams) {      // no rows: the tiles are handed back
                 ok = wait_phase(q_full, segment++ & 1, abort_flag, p.err, kErrFullWait);   // not to be two phases ahead of it later
                 if (!ok) return false;
@@ -290,31 +291,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         const float sl = fmaxf(fabsf(p.scale_log2), 1e-30f);   // above zero: a masked -inf stays one
         const uint64_t sl2 = pack_f32x2(sl, sl);
         int done = 0, loads = 0, segment = 0, mine = 0;   // steps of this stream, loads of the ring, segments, this stream's segments
-        segments([&](int head, int row0, int streams, int tile0, int tiles, int slot) {
+        segments([&](int item, int row0, int streams, int tile0, int tiles) {
             if (s >= streams) {   // no rows here; not to arrive for the next segment before this one's queries are there
                 if (lane == 0) mbar_arrive(q_full);
                 loads += 2 * tiles;
                 return __all_sync(0xffffffffu, wait_phase(q_full, segment++ & 1, abort_flag, p.err, kErrAccWait)) != 0;
             }
             ++segment;
-            const int row = row0 + s * kTcTile + r;
-            const bool real = row < rows;
-            const int t = real ? row / p.group : 0, hq = head * p.group + (real ? row - t * p.group : 0);
-            const size_t unit = (size_t)t * p.q_heads + hq;
+            // this warp's 32 rows; row = (token, query head of the kv head), unit its place in q and in the parts
+            const int head = item / p.prefix_tiles, warp_row = row0 + s * kTcTile + (warp & 3) * 32, row = warp_row + lane;
+            const int t = row < rows ? row / p.group : 0, unit = t * p.q_heads + head * p.group + (row < rows ? row - t * p.group : 0);
             {
-                // with a negative scale the queries change their sign, so that the largest product has the largest score
-                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + unit * D);
+                // Q, 16 bytes a lane along the rows.  With a negative scale the queries change their sign, so that the largest
+                // product has the largest score.
                 const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+                uint4 x[D / 8];
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    uint4 x = real ? src[c] : make_uint4(0, 0, 0, 0);
-                    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                    *reinterpret_cast<uint4 *>(base + s * kTileBytes + tile_chunk<D>(r, c, kTcTile)) = x;
+                for (int i = 0; i < D / 8; ++i) {
+                    const int rr = (i * 32 + lane) / (D / 8), c = (i * 32 + lane) % (D / 8), u = __shfl_sync(0xffffffffu, unit, rr);
+                    x[i] = warp_row + rr < rows ? reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (size_t)u * D)[c] : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const int rr = (i * 32 + lane) / (D / 8), c = (i * 32 + lane) % (D / 8);
+                    x[i].x ^= flip; x[i].y ^= flip; x[i].z ^= flip; x[i].w ^= flip;
+                    *reinterpret_cast<uint4 *>(base + s * kTileBytes + tile_chunk<D>((warp & 3) * 32 + rr, c, kTcTile)) = x[i];
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
             }
+            const int slot = (int)blockIdx.x - cut.first_block(item);
+            if (threadIdx.x == 0 && tile0 + tiles == cut.tiles) p.item_slots[item] = slot + 1;
             float ref = 0.0f, l = 0.0f;   // ref in units of log2
             for (int h = 0; h < 2 * tiles; ++h, ++done) {
                 const int buf = h & 1;
@@ -401,20 +409,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             bool ok = wait_phase(o_done + 2 * s + 1, mine++ & 1, abort_flag, p.err, kErrAccWait);
             if (!__all_sync(0xffffffffu, ok)) return false;
             tc_fence_after();
-            const size_t at = (size_t)slot * p.batch.rows * p.q_heads + unit;
-            float4 *dst = reinterpret_cast<float4 *>(p.part_o + at * D);
+            // O through shared memory (over this warp's rows of Q, whose MMAs are done), so that whole lines are written
+            constexpr int kCols = D >= 64 ? 32 : 16, kChunks = kCols / 4;
+            uint32_t high[16];   // head_dim 32: two halves of 16 columns, as its Q leaves no more room
+            uint8_t *stage = base + s * kTileBytes + (warp & 3) * 32 * D * 2;
+            const size_t at = (size_t)slot * p.batch.rows * p.q_heads;
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < D / kCols; ++c) {
                 uint32_t o[32];
-                tmem_ld32_async(to + 32 * c, o);
-                tmem_ld_wait(o);
-                if (real)
+                if constexpr (kCols == 32) {
+                    tmem_ld32_async(to + 32 * c, o);
+                    tmem_ld_wait(o);
+                } else if (c == 0) {
+                    tmem_ld32_async(to, o);
+                    tmem_ld_wait(o);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        dst[8 * c + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                                                     __uint_as_float(o[4 * i + 3]));
+                    for (int i = 0; i < 16; ++i) high[i] = o[16 + i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = high[i];
+                }
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i)
+                    *reinterpret_cast<uint4 *>(stage + lane * kCols * 4 + ((i ^ (lane & (kChunks - 1))) << 4)) =
+                        make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i) {
+                    const int rr = (i * 32 + lane) / kChunks, x = (i * 32 + lane) % kChunks, u = __shfl_sync(0xffffffffu, unit, rr);
+                    const uint4 y = *reinterpret_cast<const uint4 *>(stage + rr * kCols * 4 + ((x ^ (rr & (kChunks - 1))) << 4));
+                    if (warp_row + rr < rows) reinterpret_cast<uint4 *>(p.part_o + (at + u) * D + c * kCols)[x] = y;
+                }
+                __syncwarp();
             }
-            if (real) p.part_ml[at] = make_float2(ref, l);
+            if (row < rows) p.part_ml[at + unit] = make_float2(ref, l);
             tc_fence_before();
             return true;
         });
