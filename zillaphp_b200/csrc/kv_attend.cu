@@ -13,110 +13,373 @@ namespace {
 using namespace tc;
 
 constexpr int kTile = 64;                                 // keys of a stage
-constexpr int kSplitThreads = 160;                        // four warps that compute, one that loads
-template <int D>
-constexpr int split_stages() { return D == 128 ? 3 : D == 64 ? 4 : 6; }
-template <int D>
-constexpr int split_smem() { return split_stages<D>() * 2 * kTile * D * 2 + 1024 + 256; }
+constexpr int kSplitThreads = 128;   // four warps: a fifth that only loads would cost a quarter of an SM partition's registers
+// What one block of the two kernels below takes: a tile of rows (token-major, then the group's query heads, which share
+// the keys) and one slot of keys, of the prefix or of one sequence.
+struct SplitItem {
+    bool shared;
+    int head, row0, rows;    // kv head; first row of the tile, rows of the whole sequence (prefix: batch)
+    int first, n, len;
+    int begin, end, slot;
+    const int *pages;
+    bool empty;              // no rows, or no keys (and not to write zeros either)
+};
 
-// One block takes a tile of 16 WM rows (rows of several tokens and of the group's query heads, which share
-// the keys) and one slot of keys.  WM warps lie along the rows; the others take their part of each 64 keys
-// and are joined at the end through shared memory.  One pass with the running maximum and sum in registers:
-// S = Q K^T and O += P V by warp-level MMA, P rounded to the cache's type (half a step of 2^-8 or 2^-11 on
-// weights that average out), everything else fp32.
-// Bound by HBM where the rows are few: K and V come once, by TMA through the page list, three to six
-// stages ahead.
-template <typename T, int D, int WM>
-__global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __grid_constant__ AttendParams p) {
-    constexpr int WN = 4 / WM, KW = kTile / WN, NT = KW / 8, ST = split_stages<D>();
-    constexpr int kTileBytes = kTile * D * 2, kHalves = D == 128 ? 2 : 1, kRowBytes = D < 64 ? D * 2 : 128;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw = smem_u32(smem_raw);
-    uint8_t *base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
-    uint64_t *full = reinterpret_cast<uint64_t *>(base + ST * 2 * kTileBytes), *empty = full + ST;
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(empty + ST);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < ST; ++i) {
-            mbar_init(full + i, 1);
-            mbar_init(empty + i, 4);
-        }
-        *abort_flag = 0;
-        fence_barrier_init();
+__device__ __forceinline__ SplitItem split_item(const AttendParams &p, int item, int tile_rows) {
+    SplitItem x;
+    x.shared = item < p.prefix_items;
+    if (!x.shared) item -= p.prefix_items;
+    x.head = item % p.kv_heads;
+    item /= p.kv_heads;
+    const int tiles = x.shared ? p.prefix_tiles : p.own_tiles;
+    x.row0 = item % tiles * tile_rows;
+    item /= tiles;
+    x.first = 0;
+    x.n = p.batch.rows;
+    x.len = p.batch.prefix_len;
+    x.slot = item;
+    x.pages = p.prefix_pages;
+    int chunk = p.prefix_chunk;
+    if (!x.shared) {
+        x.slot = item % p.own_splits;
+        const int b = item / p.own_splits;
+        load_sequence(p, b, x.first, x.n, x.len);
+        x.pages = p.batch.pages + (size_t)b * p.batch.max_pages;
+        chunk = p.own_chunk;
     }
-    // Behind the tcgen05 kernel nothing here depends on that kernel's results, and it has been started only after all blocks of
-    // it found the work before them done (they wait, then allow this one): the two run side by side.  What the host's
-    // earlier kernels wrote is read past L1 (__ldcg, TMA).  The last block only waits for
-    // the tcgen05 kernel, so that this grid does not end before it: the join behind waits for this grid alone.
+    x.rows = x.n * p.group;
+    x.begin = x.slot * chunk;
+    const int last_j = p.by_group.div(max(0, min(x.rows - 1, x.row0 + tile_rows - 1)));
+    x.end = min(min(x.begin + chunk, x.len), x.shared ? x.len : own_limit(x.len, x.n, last_j));
+    x.empty = x.row0 >= x.rows || (x.begin >= x.end && !(p.direct && x.slot == 0));
+    if (!x.shared) x.slot += p.prefix_splits;
+    return x;
+}
+
+// K and V of 64-key steps by TMA, one box a lane, into a ring of ST stages.  The four warps take turns in loading the stage
+// of the step before, whose page numbers they have looked up a step ahead: a fifth warp that only loads would cost a quarter
+// of an SM partition's registers, and one of the four that loads always would hold the others up.
+template <int D, int ST>
+struct SplitRing {
+    static constexpr int kTileBytes = kTile * D * 2, kHalves = D == 128 ? 2 : 1, kRowBytes = D < 64 ? D * 2 : 128;
+    static constexpr int kBytes = ST * 2 * kTileBytes;
+    uint8_t *base;         // stage st: K at 2 st tiles, V at 2 st + 1
+    uint64_t *full, *empty;
+    volatile int *abort_flag;
+    int all, r0, half, is_v, steps, warp, lane, next_page;
+    __device__ __forceinline__ SplitRing(uint8_t *smem, int boxes) : base(smem), warp(threadIdx.x >> 5), lane(threadIdx.x & 31), next_page(0) {
+        full = reinterpret_cast<uint64_t *>(smem + kBytes);
+        empty = full + ST;
+        abort_flag = reinterpret_cast<volatile int *>(empty + ST);
+        all = boxes * kHalves * 2;   // 2 .. 16
+        r0 = lane % boxes * (kTile / boxes);
+        half = lane / boxes % kHalves;
+        is_v = lane / (boxes * kHalves);
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < ST; ++i) {
+                mbar_init(full + i, 1);
+                mbar_init(empty + i, 4);
+            }
+            *abort_flag = 0;
+            fence_barrier_init();
+        }
+    }
+    __device__ __forceinline__ void load(const AttendParams &p, int step, int at) const {
+        const int st = step % ST;
+        if (lane == 0) mbar_arrive_expect_tx(full + st, 2 * kTileBytes);
+        __syncwarp();
+        if (lane < all)
+            tma_load_2d(base + (2 * st + is_v) * kTileBytes + half * kTile * 128 + r0 * kRowBytes, is_v ? &p.v_map : &p.k_map, full + st,
+                        half * 64, at);
+    }
+    // the first ST steps, by the first warp
+    __device__ __forceinline__ void start(const AttendParams &p, const SplitItem &x) {
+        steps = x.begin < x.end ? (x.end - x.begin + kTile - 1) / kTile : 0;
+        if (warp != 0) return;
+        int at[ST];
+#pragma unroll
+        for (int i = 0; i < ST; ++i) at[i] = i < steps && lane < all ? box_row(p, x.pages, x.head, x.begin + i * kTile + r0, x.end) : 0;
+#pragma unroll
+        for (int i = 0; i < ST; ++i)
+            if (i < steps) load(p, i, at[i]);
+    }
+    // At the start of step `it`, by all warps: the warp whose turn it is loads step it - 1 + ST over step it - 1; the next
+    // one looks its page numbers up.  False: given up.
+    __device__ __forceinline__ bool refill(const AttendParams &p, const SplitItem &x, int it) {
+        const int step = it - 1 + ST, key = x.begin + step * kTile + r0;
+        if (it > 0 && step < steps && (it & 3) == warp) {
+            const int at = key < x.end ? box_row_of(p, next_page, x.head, key) : p.pages * p.kv_heads << p.page_log2;
+            if (!__all_sync(0xffffffffu, wait_phase(empty + step % ST, (step / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait))) return false;
+            load(p, step, lane < all ? at : 0);
+        }
+        if (((it + 1) & 3) == warp && lane < all && key + kTile < x.end) next_page = __ldcg(x.pages + ((key + kTile) >> p.page_log2));
+        return true;
+    }
+    __device__ __forceinline__ bool wait(const AttendParams &p, int it) const {
+        return __all_sync(0xffffffffu, wait_phase(full + it % ST, (it / ST) & 1, abort_flag, p.err, kErrFullWait)) != 0;
+    }
+    __device__ __forceinline__ void done(int it) const {   // this warp has read the step's stage
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + it % ST);
+    }
+    // A warp that gives up at step `it`: the copies in flight (steps up to it - 1 + ST) end before the block's shared memory goes.
+    __device__ __forceinline__ void drain(const AttendParams &p, int it) const {
+        if (lane == 0)
+            for (int i = max(0, it - 1); i < min(steps, it + ST); ++i)
+                if (!mbar_wait_drain(full + i % ST, (i / ST) & 1)) atomicCAS(p.err, 0, kErrDrain);
+        __syncwarp();
+    }
+};
+
+// The wait at the start.  Behind the tcgen05 kernel nothing here depends on that kernel's results, and it has been started
+// only after all blocks of it found the work before them done (they wait, then allow this one): the two run side by side.
+// What the host's earlier kernels wrote is read past L1 (__ldcg, TMA).  The last block only waits for the tcgen05 kernel,
+// so that this grid does not end before it: the join behind waits for this grid alone.  False: the block is done.
+__device__ __forceinline__ bool split_start(const AttendParams &p) {
     griddep_launch();
     if (!p.behind_tc) {
         griddep_wait();
     } else if (blockIdx.x == gridDim.x - 1) {
         griddep_wait();
-        return;
+        return false;
     }
+    return true;
+}
 
-    // the block's item: (slot, row tile, kv head) of the prefix or of one sequence
-    int item = blockIdx.x;
-    const bool shared = item < p.prefix_items;
-    if (!shared) item -= p.prefix_items;
-    const int head = item % p.kv_heads;
-    item /= p.kv_heads;
-    const int tiles = shared ? p.prefix_tiles : p.own_tiles;
-    const int tile = item % tiles;
-    item /= tiles;
-    int first = 0, n = p.batch.rows, len = p.batch.prefix_len, slot = item, chunk = p.prefix_chunk;
-    const int *pages = p.prefix_pages;
-    if (!shared) {
-        slot = item % p.own_splits;
-        const int b = item / p.own_splits;
-        load_sequence(p, b, first, n, len);
-        pages = p.batch.pages + (size_t)b * p.batch.max_pages;
-        chunk = p.own_chunk;
-    }
-    const int row0 = tile * 16 * WM, rows = n * p.group;   // rows of the item: token-major, then the group's heads
-    if (row0 >= rows) return;
-    const int last_j = min(rows - 1, row0 + 16 * WM - 1) / p.group;
-    const int begin = slot * chunk, end = min(min(begin + chunk, len), shared ? len : own_limit(len, n, last_j));
-    if (begin >= end && !(p.direct && slot == 0)) return;
-    const int steps = begin < end ? (end - begin + kTile - 1) / kTile : 0;
-    if (!shared) slot += p.prefix_splits;
+__device__ __forceinline__ void movmatrix_trans(uint32_t &d, uint32_t a) {
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+}
+
+// Few rows (up to 8 R8 = 8 .. 24 that share the keys): the products are taken with the keys as the long side, so that
+// rows are padded to 8 and not to 16, and all four warps lie along the keys (16 of each 64):
+//   S^T = K Q^T        16 keys x 8 rows an MMA, K from shared memory, Q^T in registers
+//   O^T += V^T P^T     16 of head_dim x 8 rows, V read transposed, P^T by a transposition of S^T's registers
+// A row's reference maximum follows the scores only when they pass it by 2^8, so most steps need no maximum across lanes
+// at all.  P is rounded to the cache's type (half a step of 2^-8 or 2^-11 on weights that average out), everything else is
+// fp32; the warps are joined at the end through shared memory.
+// Bound by HBM: K and V come once, by TMA through the page list, several stages ahead.
+constexpr int few_blocks(int D, int R8) { return D == 128 && R8 == 3 ? 2 : D == 32 ? 4 : 3; }
+constexpr int few_stages(int D, int R8) { return D == 128 ? (R8 == 3 ? 3 : 2) : D == 64 ? 4 : 6; }
+constexpr int few_smem(int D, int R8) { return few_stages(D, R8) * 2 * kTile * D * 2 + 1024 + 256; }
+
+template <typename T, int D, int R8>
+__global__ void __launch_bounds__(kSplitThreads, few_blocks(D, R8)) attend_few_kernel(const __grid_constant__ AttendParams p) {
+    constexpr int ST = few_stages(D, R8), kTileBytes = kTile * D * 2, kRows = 8 * R8, kPitch = D + 4;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t *base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    SplitRing<D, ST> ring(base, kTile / p.box_rows);
+    if (!split_start(p)) return;
+    const SplitItem x = split_item(p, blockIdx.x, kRows);
+    if (x.empty) return;
     __syncthreads();
-
-    if (warp == 4) {
-        const int boxes = kTile / p.box_rows, all = boxes * kHalves * 2;
-        const int r0 = lane % boxes * p.box_rows, half = lane / boxes % kHalves, is_v = lane / (boxes * kHalves);
-        bool ok = true;
-        int it = 0;
-        for (; it < steps; ++it) {
-            const int st = it % ST, at = lane < all ? box_row(p, pages, head, begin + it * kTile + r0, end) : 0;
-            ok = it < ST || wait_phase(empty + st, (it / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(full + st, 2 * kTileBytes);
-            __syncwarp();
-            if (lane < all)
-                tma_load_2d(base + (2 * st + is_v) * kTileBytes + half * kTile * 128 + r0 * kRowBytes, is_v ? &p.v_map : &p.k_map,
-                            full + st, half * 64, at);
+    ring.start(p, x);
+    const int steps = ring.steps;
+    // this warp's 16 keys of a step: the thread holds keys g, g + 8 and rows 8 i + c2, 8 i + c2 + 1 of S^T, and row 8 i + g of Q
+    const int g = lane >> 2, c2 = 2 * (lane & 3);
+    uint32_t qf[D / 16][R8][2];
+#pragma unroll
+    for (int i = 0; i < R8; ++i) {
+        const int row = x.row0 + 8 * i + g;
+        const bool real = row < x.rows;
+        const int j = real ? p.by_group.div(row) : 0, hq = x.head * p.group + (real ? row - j * p.group : 0);
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(static_cast<const T *>(p.q) + ((size_t)(x.first + j) * p.q_heads + hq) * D + c2);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            qf[k][i][0] = real ? __ldcg(src + 8 * k) : 0u;
+            qf[k][i][1] = real ? __ldcg(src + 8 * k + 4) : 0u;
         }
-        if (!ok && lane == 0)   // the copies in flight end before the block's shared memory goes
-            for (int i = max(0, it - ST); i < it; ++i)
-                if (!mbar_wait_drain(full + i % ST, (i / ST) & 1)) atomicCAS(p.err, 0, kErrDrain);
-        return;
     }
+    auto limit = [&](int i, int e) {   // keys that a row of S^T's columns sees end here
+        const int row = x.row0 + 8 * i + c2 + e;
+        return x.shared || row >= x.rows ? x.end : min(x.end, own_limit(x.len, x.n, p.by_group.div(row)));
+    };
+    const int low = x.shared ? x.end : min(x.end, own_limit(x.len, x.n, p.by_group.div(x.row0)));   // the first row sees the fewest keys
+    float o[D / 16][R8][4] = {}, m[R8][2], l[R8][2];   // m: the rows' references in units of log2, 0 before the first key
+#pragma unroll
+    for (int i = 0; i < R8; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            m[i][e] = -INFINITY;
+            l[i][e] = 0.0f;
+        }
+    const float sl = p.scale_log2;
+    int it = 0;
+    bool ok = true, open = true;   // open: some row that sees keys has no finite reference yet
+    for (; it < steps; ++it) {
+        const int st = it % ST, key0 = x.begin + it * kTile + warp * 16;
+        ok = ring.refill(p, x, it) && ring.wait(p, it);
+        if (!ok) break;
+        const uint32_t sk = smem_u32(base) + 2 * st * kTileBytes, sv = sk + kTileBytes;
+        float s[R8][4];
+#pragma unroll
+        for (int i = 0; i < R8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            uint32_t a[4];
+            ldmatrix_x4(a, sk + tile_chunk<D>(warp * 16 + (lane & 15), 2 * k + (lane >> 4), kTile));
+#pragma unroll
+            for (int i = 0; i < R8; ++i) mma_16816<T>(s[i], a, qf[k][i][0], qf[k][i][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < R8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][e] *= sl;
+        if (key0 + 16 > low) {   // keys behind some row's last
+#pragma unroll
+            for (int i = 0; i < R8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int last = limit(i, e);
+                    if (key0 + g >= last) s[i][e] = -INFINITY;
+                    if (key0 + g + 8 >= last) s[i][e + 2] = -INFINITY;
+                }
+        }
+        bool over = open;
+#pragma unroll
+        for (int i = 0; i < R8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) over |= s[i][e] > m[i][e & 1] + 8.0f;
+        if (__any_sync(0xffffffffu, over)) {
+            bool still = false;
+#pragma unroll
+            for (int i = 0; i < R8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[i][e], s[i][e + 2]);
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    const float now = fmaxf(m[i][e], top), f = now == -INFINITY ? 1.0f : ex2(m[i][e] - now);
+                    m[i][e] = now;
+                    l[i][e] *= f;
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        o[d][i][e] *= f;
+                        o[d][i][e + 2] *= f;
+                    }
+                    if (now == -INFINITY) still |= key0 < limit(i, e);
+                }
+            open = __any_sync(0xffffffffu, still);
+        }
+        uint32_t pt[R8][2];
+#pragma unroll
+        for (int i = 0; i < R8; ++i) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = ex2(s[i][e] - (m[i][e & 1] == -INFINITY ? 0.0f : m[i][e & 1]));
+                l[i][e & 1] += w[e];
+            }
+            movmatrix_trans(pt[i][0], pack2<T>(w[0], w[1]));   // keys 0-7 x rows, then keys 8-15
+            movmatrix_trans(pt[i][1], pack2<T>(w[2], w[3]));
+        }
+        if (key0 + 16 > x.end) {   // the keys behind the last: whatever their page holds, V counts as zero
+            const int from = max(0, x.end - key0);
+            for (int i = lane; i < (16 - from) * (D / 8); i += 32)
+                *reinterpret_cast<uint4 *>(base + (2 * st + 1) * kTileBytes + tile_chunk<D>(warp * 16 + from + i / (D / 8), i % (D / 8), kTile)) =
+                    make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            uint32_t a[4];
+            ldmatrix_x4_trans(a, sv + tile_chunk<D>(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * d + ((lane >> 3) & 1), kTile));
+#pragma unroll
+            for (int i = 0; i < R8; ++i) mma_16816<T>(o[d][i], a, pt[i][0], pt[i][1]);
+        }
+        ring.done(it);
+    }
+    if (!ok) ring.drain(p, it);
+    // join the warps over the stages, which all of them have read
+    float *red = reinterpret_cast<float *>(base);                              // [4][kRows][kPitch]
+    float2 *ml = reinterpret_cast<float2 *>(red + 4 * kRows * kPitch);         // [4][kRows]
+    static_assert(4 * kRows * (kPitch + 2) * 4 <= ST * 2 * kTileBytes, "the join fits the stages");
+    named_bar_sync(1, 128);
+#pragma unroll
+    for (int i = 0; i < R8; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = warp * kRows + 8 * i + c2 + e;
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], w);
+            if (g == 0) ml[r] = make_float2(m[i][e], l[i][e]);
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                red[r * kPitch + 16 * d + g] = o[d][i][e];
+                red[r * kPitch + 16 * d + g + 8] = o[d][i][e + 2];
+            }
+        }
+    named_bar_sync(1, 128);
+    if (*ring.abort_flag) return;
+    for (int i = threadIdx.x; i < min(kRows, x.rows - x.row0) * (D / 4); i += 128) {
+        const int r = i / (D / 4), c = i % (D / 4), row = x.row0 + r, j = p.by_group.div(row), hq = x.head * p.group + row - j * p.group;
+        float2 y[4];
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            y[w] = ml[w * kRows + r];
+            top = fmaxf(top, y[w].x);
+        }
+        const float use = top == -INFINITY ? 0.0f : top;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = ex2(y[w].x - use);
+            const float4 z = *reinterpret_cast<const float4 *>(red + (w * kRows + r) * kPitch + 4 * c);
+            sum += f * y[w].y;
+            acc.x += f * z.x;
+            acc.y += f * z.y;
+            acc.z += f * z.z;
+            acc.w += f * z.w;
+        }
+        const size_t at = (size_t)(x.first + j) * p.q_heads + hq;
+        if (p.direct) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + 4 * c) =
+                make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+        } else {
+            const size_t to = (size_t)x.slot * p.batch.rows * p.q_heads + at;
+            *reinterpret_cast<float4 *>(p.part_o + to * D + 4 * c) = acc;
+            if (c == 0) p.part_ml[to] = make_float2(top, sum);
+        }
+    }
+}
 
-    // this warp's 16 rows; the thread holds rows g and g + 8 of them, columns 2c, 2c + 1 of each 8
-    const int wm = warp % WM, wn = warp / WM, g = lane >> 2, c2 = 2 * (lane & 3);
-    const int row[2] = {row0 + wm * 16 + g, row0 + wm * 16 + g + 8};
+// Many rows (64 a tile): four warps along the rows, each with all keys of a step.  S = Q K^T and O += P V by warp-level
+// MMA, one pass with the running maximum and sum in registers, the same roundings and lazy rescale as above.
+// Compute bound: K and V are read from shared memory by each of the four warps.
+constexpr int kManyRows = 64, kManyBlocks = 3;
+constexpr int many_stages(int D) { return D == 128 ? 2 : D == 64 ? 4 : 6; }
+constexpr int many_smem(int D) { return many_stages(D) * 2 * kTile * D * 2 + 1024 + 256; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kSplitThreads, kManyBlocks) attend_many_kernel(const __grid_constant__ AttendParams p) {
+    constexpr int NT = kTile / 8, ST = many_stages(D), kTileBytes = kTile * D * 2;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t *base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    SplitRing<D, ST> ring(base, kTile / p.box_rows);
+    if (!split_start(p)) return;
+    const SplitItem x = split_item(p, blockIdx.x, kManyRows);
+    if (x.empty) return;
+    __syncthreads();
+    ring.start(p, x);
+    const int steps = ring.steps;
+    // this warp's 16 rows; the thread holds rows g and g + 8 of them, columns c2, c2 + 1 of each 8
+    const int g = lane >> 2, c2 = 2 * (lane & 3);
+    const int row[2] = {x.row0 + warp * 16 + g, x.row0 + warp * 16 + g + 8};
     int limit[2];
     uint32_t qf[D / 16][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const bool real = row[i] < rows;
-        const int j = real ? row[i] / p.group : 0, hq = head * p.group + row[i] - j * p.group;
-        limit[i] = shared ? end : min(end, own_limit(len, n, j));
-        const uint32_t *src = reinterpret_cast<const uint32_t *>(static_cast<const T *>(p.q) +
-                                                                 ((size_t)(first + j) * p.q_heads + (real ? hq : 0)) * D + c2);
+        const bool real = row[i] < x.rows;
+        const int j = real ? p.by_group.div(row[i]) : 0, hq = x.head * p.group + (real ? row[i] - j * p.group : 0);
+        limit[i] = x.shared || !real ? x.end : min(x.end, own_limit(x.len, x.n, j));
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(static_cast<const T *>(p.q) + ((size_t)(x.first + j) * p.q_heads + hq) * D + c2);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
             qf[k][i] = real ? __ldcg(src + 8 * k) : 0u;
@@ -124,12 +387,13 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
         }
     }
     float o[D / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const int low = min(limit[0], limit[1]);
+    const int low = x.shared ? x.end : min(x.end, own_limit(x.len, x.n, p.by_group.div(min(x.rows - 1, x.row0 + warp * 16))));
+    int it = 0;
     bool ok = true;
-    for (int it = 0; it < steps; ++it) {
-        const int st = it % ST, key0 = begin + it * kTile + wn * KW;
-        ok = wait_phase(full + st, (it / ST) & 1, abort_flag, p.err, kErrFullWait);
-        if (!__all_sync(0xffffffffu, ok)) break;
+    for (; it < steps; ++it) {
+        const int st = it % ST, key0 = x.begin + it * kTile;
+        ok = ring.refill(p, x, it) && ring.wait(p, it);
+        if (!ok) break;
         const uint32_t sk = smem_u32(base) + 2 * st * kTileBytes, sv = sk + kTileBytes;
         float s[NT][4];
 #pragma unroll
@@ -141,34 +405,45 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < NT / 2; ++i) {
                 uint32_t b[4];
-                ldmatrix_x4(b, sk + tile_chunk<D>(wn * KW + 16 * i + ((lane >> 4) << 3) + (lane & 7), 2 * k + ((lane >> 3) & 1), kTile));
+                ldmatrix_x4(b, sk + tile_chunk<D>(16 * i + ((lane >> 4) << 3) + (lane & 7), 2 * k + ((lane >> 3) & 1), kTile));
                 mma_16816<T>(s[2 * i], qf[k], b[0], b[1]);
                 mma_16816<T>(s[2 * i + 1], qf[k], b[2], b[3]);
             }
-        float top[2] = {m[0], m[1]};
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[i][e] *= p.scale_log2;
-                if (key0 + KW > low && key0 + 8 * i + c2 + (e & 1) >= limit[e >> 1]) s[i][e] = -INFINITY;
-                top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
-            }
-        float use[2];
+            for (int e = 0; e < 4; ++e) s[i][e] *= p.scale_log2;
+        if (key0 + kTile > low) {   // keys behind some row's last
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (key0 + 8 * i + c2 + (e & 1) >= limit[e >> 1]) s[i][e] = -INFINITY;
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
             top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-            use[i] = top[i] == -INFINITY ? 0.0f : top[i];   // a row without keys so far
-            const float f = ex2(m[i] - use[i]);
-            m[i] = top[i];
-            l[i] *= f;
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
 #pragma unroll
-            for (int d = 0; d < D / 8; ++d) {
-                o[d][2 * i] *= f;
-                o[d][2 * i + 1] *= f;
+            for (int i = 0; i < 2; ++i) {
+                const float now = fmaxf(m[i], top[i]), f = now == -INFINITY ? 1.0f : ex2(m[i] - now);
+                m[i] = now;
+                l[i] *= f;
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d) {
+                    o[d][2 * i] *= f;
+                    o[d][2 * i + 1] *= f;
+                }
             }
         }
+        const float use[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};   // a row without keys so far
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -176,14 +451,11 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
                 s[i][e] = ex2(s[i][e] - use[e >> 1]);
                 l[e >> 1] += s[i][e];
             }
-        if (key0 + KW > end) {   // the rows behind the last key: whatever their page holds, V counts as zero
-            const int from = max(0, end - key0);
-            for (int x = lane; x < (KW - from) * (D / 8); x += 32) {
-                const int r = wn * KW + from + x / (D / 8);
-                *reinterpret_cast<uint4 *>(base + (2 * st + 1) * kTileBytes + tile_chunk<D>(r, x % (D / 8), kTile)) = make_uint4(0, 0, 0, 0);
-            }
-            if constexpr (WM > 1) named_bar_sync(2 + wn, 32 * WM);   // the warps that share these keys write the same zeros
-            else __syncwarp();
+        if (key0 + kTile > x.end) {   // the keys behind the last: whatever their page holds, V counts as zero
+            const int from = x.end - key0;   // each warp writes the same zeros before it reads them
+            for (int i = lane; i < (kTile - from) * (D / 8); i += 32)
+                *reinterpret_cast<uint4 *>(base + (2 * st + 1) * kTileBytes + tile_chunk<D>(from + i / (D / 8), i % (D / 8), kTile)) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
         }
 #pragma unroll
         for (int i = 0; i < NT / 2; ++i) {
@@ -192,78 +464,29 @@ __global__ void __launch_bounds__(kSplitThreads) attend_split_kernel(const __gri
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
                 uint32_t b[4];
-                ldmatrix_x4_trans(b, sv + tile_chunk<D>(wn * KW + 16 * i + (lane & 15), 2 * d + (lane >> 4), kTile));
+                ldmatrix_x4_trans(b, sv + tile_chunk<D>(16 * i + (lane & 15), 2 * d + (lane >> 4), kTile));
                 mma_16816<T>(o[2 * d], a, b[0], b[1]);
                 mma_16816<T>(o[2 * d + 1], a, b[2], b[3]);
             }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty + st);
+        ring.done(it);
     }
+    if (!ok) ring.drain(p, it);
+    if (!ok) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    }
-    if constexpr (WN > 1) {   // join the warps that took the same rows: over the stages, which all warps have read
-        constexpr int kPitch = D + 4;
-        float *red = reinterpret_cast<float *>(base);                      // [WN - 1][16 WM][kPitch]
-        float2 *ml = reinterpret_cast<float2 *>(red + (WN - 1) * 16 * WM * kPitch);
-        static_assert(((WN - 1) * 16 * WM * (kPitch + 2)) * 4 <= split_stages<D>() * 2 * kTileBytes, "the join fits the stages");
-        named_bar_sync(1, 128);
-        if (wn > 0) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = ((wn - 1) * WM + wm) * 16 + g + 8 * i;
-                if ((lane & 3) == 0) ml[r] = make_float2(m[i], l[i]);
-#pragma unroll
-                for (int d = 0; d < D / 8; ++d)
-                    *reinterpret_cast<float2 *>(red + r * kPitch + 8 * d + c2) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-            }
-        }
-        named_bar_sync(1, 128);
-        if (wn > 0) return;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float top = m[i];
-#pragma unroll
-            for (int w = 0; w < WN - 1; ++w) top = fmaxf(top, ml[(w * WM + wm) * 16 + g + 8 * i].x);
-            const float use = top == -INFINITY ? 0.0f : top, f = ex2(m[i] - use);
-            m[i] = top;
-            l[i] *= f;
-#pragma unroll
-            for (int d = 0; d < D / 8; ++d) {
-                o[d][2 * i] *= f;
-                o[d][2 * i + 1] *= f;
-            }
-#pragma unroll
-            for (int w = 0; w < WN - 1; ++w) {
-                const int r = (w * WM + wm) * 16 + g + 8 * i;
-                const float2 x = ml[r];
-                const float fw = ex2(x.x - use);
-                l[i] += fw * x.y;
-#pragma unroll
-                for (int d = 0; d < D / 8; ++d) {
-                    const float2 y = *reinterpret_cast<const float2 *>(red + r * kPitch + 8 * d + c2);
-                    o[d][2 * i] += fw * y.x;
-                    o[d][2 * i + 1] += fw * y.y;
-                }
-            }
-        }
-    }
-    if (*abort_flag) return;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (row[i] >= rows) continue;
-        const int j = row[i] / p.group, hq = head * p.group + row[i] - j * p.group;
-        const size_t at = (size_t)(first + j) * p.q_heads + hq;
+        if (row[i] >= x.rows) continue;
+        const int j = p.by_group.div(row[i]), hq = x.head * p.group + row[i] - j * p.group;
+        const size_t at = (size_t)(x.first + j) * p.q_heads + hq;
         if (p.direct) {
             const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
             uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out) + at * D + c2);
 #pragma unroll
             for (int d = 0; d < D / 8; ++d) dst[4 * d] = pack2<T>(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
         } else {
-            const size_t to = (size_t)slot * p.batch.rows * p.q_heads + at;
+            const size_t to = (size_t)x.slot * p.batch.rows * p.q_heads + at;
             float *dst = p.part_o + to * D + c2;
 #pragma unroll
             for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2 *>(dst + 8 * d) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
@@ -288,7 +511,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     griddep_wait();
     int front = p.prefix_splits;   // the prefix's slots come first
     if (p.tc_blocks && unit < units) {
-        const int head = hq / p.group, row = t * p.group + hq - head * p.group;
+        const int head = p.by_group.div(hq), row = t * p.group + hq - head * p.group;
         front = p.item_slots[head * p.prefix_tiles + row / (2 * kTcTile)];
     }
     __syncthreads();
@@ -342,14 +565,20 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
 
 // ---------------------------------------------------------------- plan
 struct Plan {
-    int tc_blocks;          // > 0: the prefix on tcgen05, by this many blocks
-    int own_wm, prefix_wm;
+    int tc_blocks;             // > 0: the prefix on tcgen05, by this many blocks
+    int own_form, prefix_form; // 8-row tiles of the few-rows kernel, 0: the many-rows kernel
     int own_tiles, prefix_tiles, own_chunk, own_splits, prefix_chunk, prefix_splits;
     bool direct;
     size_t units, part_floats;   // rows * q_heads; floats of the parts
 };
 
-int row_warps(long long rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// The few-rows kernel takes up to 24 rows; with 40 (eight heads, five tokens, head_dim 64) its accumulators fill the
+// register file and the many-rows kernel is faster (18.6 us against 24.9 for 64 sequences of 513 keys).
+int row_form(long long rows) {
+    return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 0;
+}
+int form_rows(int form) { return form ? 8 * form : kManyRows; }
+int form_blocks(int head_dim, int form) { return form ? few_blocks(head_dim, form) : kManyBlocks; }
 
 // Rows that share the prefix's keys from which it goes to tcgen05.
 constexpr int kTcRows = 64;
@@ -374,23 +603,26 @@ int choose_tc_blocks(const KvCache &c, long long units, double own_bytes) {
     return best;
 }
 
-// Row tiles of 16, 32 or 64 rows by the rows that share the keys, and slots of whole 64-key stages such
-// that all blocks together are about `kWaves` rounds of two blocks an SM: fewer would leave SMs idle, more would
-// add parts to write and join.
+// Row tiles by the rows that share the keys, and slots of whole 64-key steps: as many blocks as fit the machine at least,
+// of four steps if there are enough, and about `kWaves` rounds of them where there are many (longer ones leave SMs idle
+// at the end, shorter ones add starts, parts to write and to join).
 Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_len, int max_new, int max_len) {
-    constexpr int kWaves = 2;
+    constexpr int kWaves = 6;
     Plan p;
     const int group = q_heads / c.kv_heads;
     const long long own_rows = (long long)max_new * group, prefix_rows = (long long)rows * group;
     const bool tc = prefix_rows > kTcRows && prefix_len > 0;
-    p.own_wm = row_warps(own_rows);
-    p.prefix_wm = row_warps(prefix_rows);
-    p.own_tiles = (int)((own_rows + 16 * p.own_wm - 1) / (16 * p.own_wm));
-    const int tile_rows = tc ? 2 * kTcTile : 16 * p.prefix_wm;
+    p.own_form = row_form(own_rows);
+    p.prefix_form = row_form(prefix_rows);
+    // one launch where the own keys are few (8 MB), in the prefix's form
+    if (!tc && 4LL * batch * max_len * c.kv_heads * c.head_dim < (8LL << 20)) p.own_form = p.prefix_form;
+    p.own_tiles = (int)((own_rows + form_rows(p.own_form) - 1) / form_rows(p.own_form));
+    const int tile_rows = tc ? 2 * kTcTile : form_rows(p.prefix_form);
     p.prefix_tiles = (int)((prefix_rows + tile_rows - 1) / tile_rows);
     const long long own_steps = (max_len + kTile - 1) / kTile, prefix_steps = (prefix_len + kTile - 1) / kTile;
     const long long total = c.kv_heads * (own_steps * batch * p.own_tiles + (tc ? 0 : prefix_steps * p.prefix_tiles));
-    const long long per = std::max<long long>(1, total / (2LL * kWaves * sm_count()));
+    const long long fit = (long long)form_blocks(c.head_dim, p.own_form) * sm_count();
+    const long long per = std::max(std::min(4LL, std::max(1LL, total / fit)), total / (kWaves * fit));
     p.own_chunk = (int)std::min(per, std::max(1LL, own_steps)) * kTile;
     p.own_splits = (int)((max_len + p.own_chunk - 1) / p.own_chunk);
     p.prefix_chunk = (int)std::min(per, std::max(1LL, prefix_steps)) * kTile;
@@ -422,21 +654,29 @@ int allow_smem(K kernel, int bytes, bool (&set)[64], const char *name) {
     return kOk;
 }
 
-template <typename T, int D, int WM>
-int launch_split(const AttendParams &p, long long blocks, const char *name) {
-    static bool set[64] = {};
-    if (int rc = allow_smem(attend_split_kernel<T, D, WM>, split_smem<D>(), set, name)) return rc;
-    if (blocks > 0x7fffffffLL) return fail(kBadArg, "%s: %lld blocks are too many", name, blocks);
-    launch_pdl(attend_split_kernel<T, D, WM>, dim3((unsigned)blocks), dim3(kSplitThreads), split_smem<D>(), p);
+template <typename K>
+int launch_blocks(K kernel, const AttendParams &p, long long blocks, int smem, bool (&set)[64], const char *name) {
+    if (blocks >= 0x7fffffffLL) return fail(kBadArg, "%s: %lld blocks are too many", name, blocks);
+    if (int rc = allow_smem(kernel, smem, set, name)) return rc;
+    launch_pdl(kernel, dim3((unsigned)(blocks + (p.behind_tc ? 1 : 0))), dim3(kSplitThreads), smem, p);
     ZB_LAUNCH_CHECK(name);
     return kOk;
 }
 
+template <typename T, int D, int R8>
+int launch_few(const AttendParams &p, long long blocks, const char *name) {
+    static bool set[64] = {};
+    return launch_blocks(attend_few_kernel<T, D, R8>, p, blocks, few_smem(D, R8), set, name);
+}
+
 template <typename T, int D>
-int run_split(const AttendParams &p, int wm, long long blocks, const char *name) {
+int run_split(const AttendParams &p, int form, long long blocks, const char *name) {
     if (blocks == 0) return kOk;
-    return wm == 1 ? launch_split<T, D, 1>(p, blocks, name)
-                   : wm == 2 ? launch_split<T, D, 2>(p, blocks, name) : launch_split<T, D, 4>(p, blocks, name);
+    if (form == 1) return launch_few<T, D, 1>(p, blocks, name);
+    if (form == 2) return launch_few<T, D, 2>(p, blocks, name);
+    if (form == 3) return launch_few<T, D, 3>(p, blocks, name);
+    static bool set[64] = {};
+    return launch_blocks(attend_many_kernel<T, D>, p, blocks, many_smem(D), set, name);
 }
 
 template <typename T, int D>
@@ -450,15 +690,15 @@ int run(AttendParams p, const Plan &plan, const char *name) {
         launch_pdl(attend_tc_kernel<T, D>, dim3(plan.tc_blocks), dim3(kTcThreads), tc_smem<D>(), p);
         ZB_LAUNCH_CHECK(name);
         p.behind_tc = 1;
-        if (int rc = run_split<T, D>(p, plan.own_wm, own ? own + 1 : 0, name)) return rc;
-    } else if (plan.own_wm == plan.prefix_wm) {
+        if (int rc = run_split<T, D>(p, plan.own_form, own, name)) return rc;
+    } else if (plan.own_form == plan.prefix_form) {
         p.prefix_items = (int)prefix;
-        if (int rc = run_split<T, D>(p, plan.own_wm, prefix + own, name)) return rc;
+        if (int rc = run_split<T, D>(p, plan.own_form, prefix + own, name)) return rc;
     } else {
         p.prefix_items = (int)prefix;
-        if (int rc = run_split<T, D>(p, plan.prefix_wm, prefix, name)) return rc;
+        if (int rc = run_split<T, D>(p, plan.prefix_form, prefix, name)) return rc;
         p.prefix_items = 0;
-        if (int rc = run_split<T, D>(p, plan.own_wm, own, name)) return rc;
+        if (int rc = run_split<T, D>(p, plan.own_form, own, name)) return rc;
     }
     if (p.direct) return kOk;
     launch_pdl(attend_join_kernel<T, D>, dim3((unsigned)((plan.units + 7) / 8)), dim3(256), 0, p);
@@ -540,6 +780,7 @@ int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int 
     p.q_heads = q_heads;
     p.kv_heads = c->kv_heads;
     p.group = q_heads / c->kv_heads;
+    p.by_group = FastDiv(p.group);
     p.page_log2 = c->page_log2;
     p.pages = c->pages;
     p.box_rows = c->box_rows;

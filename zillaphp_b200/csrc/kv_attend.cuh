@@ -24,6 +24,7 @@ struct AttendParams {
     KvBatch batch;
     const int *prefix_pages;
     int q_heads, kv_heads, group, page_log2, pages, box_rows;
+    FastDiv by_group;   // rows are token-major, then the group's heads
     int max_new, max_len;
     int prefix_splits, prefix_chunk, own_splits, own_chunk;   // slots, and keys of a slot
     int prefix_tiles, own_tiles;                              // row tiles of this launch
@@ -70,17 +71,19 @@ __device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int 
     }
 }
 
-// The TMA row coordinate of the box at `key` of a page list: the cache's end (a box of zeros) behind
-// `end` and for a page number outside the cache, which is recorded.
-__device__ __forceinline__ int box_row(const AttendParams &p, const int *pages, int kv_head, int key, int end) {
-    const int none = p.pages * p.kv_heads << p.page_log2;
-    if (key >= end) return none;
-    const int id = __ldcg(pages + (key >> p.page_log2));
+// The TMA row coordinate of the box at `key` in page `id`: the cache's end (a box of zeros) for a page number outside the
+// cache, which is recorded.
+__device__ __forceinline__ int box_row_of(const AttendParams &p, int id, int kv_head, int key) {
     if (id < 0 || id >= p.pages) {
         atomicCAS(p.err, 0, kErrKvPage);
-        return none;
+        return p.pages * p.kv_heads << p.page_log2;
     }
     return ((id * p.kv_heads + kv_head) << p.page_log2) + (key & ((1 << p.page_log2) - 1));
+}
+// The same with the page number looked up; behind `end` the cache's end too.
+__device__ __forceinline__ int box_row(const AttendParams &p, const int *pages, int kv_head, int key, int end) {
+    if (key >= end) return p.pages * p.kv_heads << p.page_log2;
+    return box_row_of(p, __ldcg(pages + (key >> p.page_log2)), kv_head, key);
 }
 
 // tc::mbar_wait with the clock read only after 64 failed tries: reading %globaltimer between the first two tries delays

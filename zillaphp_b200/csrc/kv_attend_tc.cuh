@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             ++segment;
             // this warp's 32 rows; row = (token, query head of the kv head), unit its place in q and in the parts
             const int head = item / p.prefix_tiles, warp_row = row0 + s * kTcTile + (warp & 3) * 32, row = warp_row + lane;
-            const int t = row < rows ? row / p.group : 0, unit = t * p.q_heads + head * p.group + (row < rows ? row - t * p.group : 0);
+            const int t = row < rows ? p.by_group.div(row) : 0, unit = t * p.q_heads + head * p.group + (row < rows ? row - t * p.group : 0);
             {
                 // Q, 16 bytes a lane along the rows.  With a negative scale the queries change their sign, so that the largest
                 // product has the largest score.
