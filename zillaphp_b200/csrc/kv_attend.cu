@@ -495,12 +495,13 @@ __global__ void __launch_bounds__(kSplitThreads, kManyBlocks) attend_many_kernel
     }
 }
 
-// The join: one warp a (row, query head), each lane D / 32 columns.  Reads the slots' parts once, mostly from L2, eight
-// slots at a time (their addresses do not depend on their maxima, so all loads of a row are on the way together); a row
+// The join: one warp a (row, query head), each lane D / 32 columns.  Reads the slots' parts once, mostly from L2, BATCH
+// slots at a time (their addresses do not depend on their maxima, so the loads of a batch are on the way together): eight
+// where few blocks wait for the latency of many slots, four (and twice the blocks an SM) where the rows are many.  A row
 // of no sequence is left as it is, a row without keys becomes zero.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p) {
-    constexpr int C = D / 32, kBatch = 8;
+template <typename T, int D, int BATCH>
+__global__ void __launch_bounds__(256, BATCH == 4 ? 5 : 2) attend_join_kernel(const __grid_constant__ AttendParams p) {
+    constexpr int C = D / 32, kBatch = BATCH;
     __shared__ int owner[8], own_slots[8];   // of the block's tokens, eight at most
     griddep_launch();
     const int tid = threadIdx.x, lane = tid & 31;
@@ -607,7 +608,7 @@ int choose_tc_blocks(const KvCache &c, long long units, double own_bytes) {
 // of four steps if there are enough, and about `kWaves` rounds of them where there are many (longer ones leave SMs idle
 // at the end, shorter ones add starts, parts to write and to join).
 Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_len, int max_new, int max_len) {
-    constexpr int kWaves = 6;
+    constexpr int kWaves = 3;
     Plan p;
     const int group = q_heads / c.kv_heads;
     const long long own_rows = (long long)max_new * group, prefix_rows = (long long)rows * group;
@@ -701,7 +702,9 @@ int run(AttendParams p, const Plan &plan, const char *name) {
         if (int rc = run_split<T, D>(p, plan.own_form, own, name)) return rc;
     }
     if (p.direct) return kOk;
-    launch_pdl(attend_join_kernel<T, D>, dim3((unsigned)((plan.units + 7) / 8)), dim3(256), 0, p);
+    const dim3 grid((unsigned)((plan.units + 7) / 8));
+    if (grid.x <= 2u * sm_count()) launch_pdl(attend_join_kernel<T, D, 8>, grid, dim3(256), 0, p);
+    else launch_pdl(attend_join_kernel<T, D, 4>, grid, dim3(256), 0, p);
     ZB_LAUNCH_CHECK(name);
     return kOk;
 }
