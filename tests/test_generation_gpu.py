@@ -250,6 +250,16 @@ def test_attend_loose_bounds(bufs, dtype):
     run_attend(bufs, dtype, [1, 3], [20, 300], 8, 2, 128, 16, 100, 1, max_new=9, max_len=1000, max_pages=80)
 
 
+@pytest.mark.parametrize("dtype,dim,hq,hk,page,prefix,new,longest", [
+    ("bf16", 32, 4, 4, 16, 96, [1] * 16, 32), ("fp16", 64, 8, 2, 16, 5, [2, 1, 0, 3], 64), ("bf16", 128, 24, 1, 128, 65, [1, 3], 100),
+    ("fp16", 128, 4, 2, 32, 130, [4] * 230, 90),          # a prefix in front of many sequences' own keys
+    ("bf16", 64, 16, 2, 64, 256, [5, 1] * 120, 70), ("bf16", 128, 3, 3, 16, 1, [2, 1] * 90, 257), ("bf16", 32, 40, 1, 16, 63, [1] * 4, 0)])
+def test_attend_short_prefix(bufs, dtype, dim, hq, hk, page, prefix, new, longest):
+    """Short prefixes: each block runs over the prefix and its sequence's own keys, no parts are joined."""
+    length = [min(longest, n + (37 * i) % (longest + 1)) for i, n in enumerate(new)]
+    run_attend(bufs, dtype, new, length, hq, hk, dim, page, prefix, 2, max_len=max(longest, 1), max_pages=-(-max(longest, 1) // page))
+
+
 def test_attend_scales(bufs):
     run_attend(bufs, "bf16", [1, 2], [100, 70], 4, 2, 64, 16, 90, scale=-0.3)
     run_attend(bufs, "bf16", [1, 2], [100, 70], 4, 2, 64, 16, 90, scale=0.0)

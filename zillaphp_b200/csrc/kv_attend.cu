@@ -21,6 +21,7 @@ struct SplitItem {
     int head, row0, rows;    // kv head; first row of the tile, rows of the whole sequence (prefix: batch)
     int first, n, len;
     int begin, end, slot;
+    int front;               // steps over the prefix in front of the own keys (one block takes all keys of its rows)
     const int *pages;
     bool empty;              // no rows, or no keys (and not to write zeros either)
 };
@@ -51,6 +52,7 @@ __device__ __forceinline__ SplitItem split_item(const AttendParams &p, int item,
     x.begin = x.slot * chunk;
     const int last_j = p.by_group.div(max(0, min(x.rows - 1, x.row0 + tile_rows - 1)));
     x.end = min(min(x.begin + chunk, x.len), x.shared ? x.len : own_limit(x.len, x.n, last_j));
+    x.front = x.shared ? 0 : p.front_steps;
     x.empty = x.row0 >= x.rows || (x.begin >= x.end && !(p.direct && x.slot == 0));
     if (!x.shared) x.slot += p.prefix_splits;
     return x;
@@ -92,13 +94,23 @@ struct SplitRing {
             tma_load_2d(base + (2 * st + is_v) * kTileBytes + half * kTile * 128 + r0 * kRowBytes, is_v ? &p.v_map : &p.k_map, full + st,
                         half * 64, at);
     }
+    // a step's first key, in the prefix or among the item's own, and the end of its keys
+    static __device__ __forceinline__ int first_key(const SplitItem &x, int step) {
+        return step < x.front ? step * kTile : x.begin + (step - x.front) * kTile;
+    }
+    static __device__ __forceinline__ int end_of(const AttendParams &p, const SplitItem &x, int step) {
+        return step < x.front ? p.batch.prefix_len : x.end;
+    }
     // the first ST steps, by the first warp
     __device__ __forceinline__ void start(const AttendParams &p, const SplitItem &x) {
-        steps = x.begin < x.end ? (x.end - x.begin + kTile - 1) / kTile : 0;
+        steps = x.front + (x.begin < x.end ? (x.end - x.begin + kTile - 1) / kTile : 0);
         if (warp != 0) return;
         int at[ST];
 #pragma unroll
-        for (int i = 0; i < ST; ++i) at[i] = i < steps && lane < all ? box_row(p, x.pages, x.head, x.begin + i * kTile + r0, x.end) : 0;
+        for (int i = 0; i < ST; ++i) {
+            const int key = first_key(x, i) + r0;
+            at[i] = i < steps && lane < all ? box_row(p, i < x.front ? p.prefix_pages : x.pages, x.head, key, end_of(p, x, i)) : 0;
+        }
 #pragma unroll
         for (int i = 0; i < ST; ++i)
             if (i < steps) load(p, i, at[i]);
@@ -106,13 +118,17 @@ struct SplitRing {
     // At the start of step `it`, by all warps: the warp whose turn it is loads step it - 1 + ST over step it - 1; the next
     // one looks its page numbers up.  False: given up.
     __device__ __forceinline__ bool refill(const AttendParams &p, const SplitItem &x, int it) {
-        const int step = it - 1 + ST, key = x.begin + step * kTile + r0;
+        const int step = it - 1 + ST;
         if (it > 0 && step < steps && (it & 3) == warp) {
-            const int at = key < x.end ? box_row_of(p, next_page, x.head, key) : p.pages * p.kv_heads << p.page_log2;
+            const int key = first_key(x, step) + r0;
+            const int at = key < end_of(p, x, step) ? box_row_of(p, next_page, x.head, key) : p.pages * p.kv_heads << p.page_log2;
             if (!__all_sync(0xffffffffu, wait_phase(empty + step % ST, (step / ST - 1) & 1, abort_flag, p.err, kErrEmptyWait))) return false;
             load(p, step, lane < all ? at : 0);
         }
-        if (((it + 1) & 3) == warp && lane < all && key + kTile < x.end) next_page = __ldcg(x.pages + ((key + kTile) >> p.page_log2));
+        if (((it + 1) & 3) == warp && lane < all && step + 1 < steps) {
+            const int key = first_key(x, step + 1) + r0;
+            if (key < end_of(p, x, step + 1)) next_page = __ldcg((step + 1 < x.front ? p.prefix_pages : x.pages) + (key >> p.page_log2));
+        }
         return true;
     }
     __device__ __forceinline__ bool wait(const AttendParams &p, int it) const {
@@ -208,7 +224,8 @@ __global__ void __launch_bounds__(kSplitThreads, few_blocks(D, R8)) attend_few_k
     int it = 0;
     bool ok = true, open = true;   // open: some row that sees keys has no finite reference yet
     for (; it < steps; ++it) {
-        const int st = it % ST, key0 = x.begin + it * kTile + warp * 16;
+        const int st = it % ST, key0 = ring.first_key(x, it) + warp * 16, end = ring.end_of(p, x, it);
+        const bool all_see = it < x.front;   // every row sees the prefix
         ok = ring.refill(p, x, it) && ring.wait(p, it);
         if (!ok) break;
         const uint32_t sk = smem_u32(base) + 2 * st * kTileBytes, sv = sk + kTileBytes;
@@ -228,12 +245,12 @@ __global__ void __launch_bounds__(kSplitThreads, few_blocks(D, R8)) attend_few_k
         for (int i = 0; i < R8; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[i][e] *= sl;
-        if (key0 + 16 > low) {   // keys behind some row's last
+        if (key0 + 16 > (all_see ? end : low)) {   // keys behind some row's last
 #pragma unroll
             for (int i = 0; i < R8; ++i)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int last = limit(i, e);
+                    const int last = all_see ? end : limit(i, e);
                     if (key0 + g >= last) s[i][e] = -INFINITY;
                     if (key0 + g + 8 >= last) s[i][e + 2] = -INFINITY;
                 }
@@ -260,7 +277,7 @@ __global__ void __launch_bounds__(kSplitThreads, few_blocks(D, R8)) attend_few_k
                         o[d][i][e] *= f;
                         o[d][i][e + 2] *= f;
                     }
-                    if (now == -INFINITY) still |= key0 < limit(i, e);
+                    if (now == -INFINITY) still |= key0 < (all_see ? end : limit(i, e));
                 }
             open = __any_sync(0xffffffffu, still);
         }
@@ -276,11 +293,12 @@ __global__ void __launch_bounds__(kSplitThreads, few_blocks(D, R8)) attend_few_k
             movmatrix_trans(pt[i][0], pack2<T>(w[0], w[1]));   // keys 0-7 x rows, then keys 8-15
             movmatrix_trans(pt[i][1], pack2<T>(w[2], w[3]));
         }
-        if (key0 + 16 > x.end) {   // the keys behind the last: whatever their page holds, V counts as zero
-            const int from = max(0, x.end - key0);
+        if (key0 + 16 > end) {   // the keys behind the last: whatever their page holds, V counts as zero
+            const int from = max(0, end - key0);
             for (int i = lane; i < (16 - from) * (D / 8); i += 32)
                 *reinterpret_cast<uint4 *>(base + (2 * st + 1) * kTileBytes + tile_chunk<D>(warp * 16 + from + i / (D / 8), i % (D / 8), kTile)) =
                     make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();   // before a later copy into this stage
             __syncwarp();
         }
 #pragma unroll
@@ -391,7 +409,8 @@ __global__ void __launch_bounds__(kSplitThreads, kManyBlocks) attend_many_kernel
     int it = 0;
     bool ok = true;
     for (; it < steps; ++it) {
-        const int st = it % ST, key0 = x.begin + it * kTile;
+        const int st = it % ST, key0 = ring.first_key(x, it), end = ring.end_of(p, x, it);
+        const bool all_see = it < x.front;   // every row sees the prefix
         ok = ring.refill(p, x, it) && ring.wait(p, it);
         if (!ok) break;
         const uint32_t sk = smem_u32(base) + 2 * st * kTileBytes, sv = sk + kTileBytes;
@@ -413,12 +432,12 @@ __global__ void __launch_bounds__(kSplitThreads, kManyBlocks) attend_many_kernel
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[i][e] *= p.scale_log2;
-        if (key0 + kTile > low) {   // keys behind some row's last
+        if (key0 + kTile > (all_see ? end : low)) {   // keys behind some row's last
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (key0 + 8 * i + c2 + (e & 1) >= limit[e >> 1]) s[i][e] = -INFINITY;
+                    if (key0 + 8 * i + c2 + (e & 1) >= (all_see ? end : limit[e >> 1])) s[i][e] = -INFINITY;
         }
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -451,10 +470,11 @@ __global__ void __launch_bounds__(kSplitThreads, kManyBlocks) attend_many_kernel
                 s[i][e] = ex2(s[i][e] - use[e >> 1]);
                 l[e >> 1] += s[i][e];
             }
-        if (key0 + kTile > x.end) {   // the keys behind the last: whatever their page holds, V counts as zero
-            const int from = x.end - key0;   // each warp writes the same zeros before it reads them
+        if (key0 + kTile > end) {   // the keys behind the last: whatever their page holds, V counts as zero
+            const int from = end - key0;   // each warp writes the same zeros before it reads them
             for (int i = lane; i < (kTile - from) * (D / 8); i += 32)
                 *reinterpret_cast<uint4 *>(base + (2 * st + 1) * kTileBytes + tile_chunk<D>(from + i / (D / 8), i % (D / 8), kTile)) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();   // before a later copy into this stage
             __syncwarp();
         }
 #pragma unroll
@@ -569,6 +589,7 @@ struct Plan {
     int tc_blocks;             // > 0: the prefix on tcgen05, by this many blocks
     int own_form, prefix_form; // 8-row tiles of the few-rows kernel, 0: the many-rows kernel
     int own_tiles, prefix_tiles, own_chunk, own_splits, prefix_chunk, prefix_splits;
+    int front_steps;           // > 0: no shared work, every block runs over the prefix in front of its own keys
     bool direct;
     size_t units, part_floats;   // rows * q_heads; floats of the parts
 };
@@ -612,15 +633,33 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
     Plan p;
     const int group = q_heads / c.kv_heads;
     const long long own_rows = (long long)max_new * group, prefix_rows = (long long)rows * group;
-    const bool tc = prefix_rows > kTcRows && prefix_len > 0;
+    const long long own_steps = (max_len + kTile - 1) / kTile, prefix_steps = (prefix_len + kTile - 1) / kTile;
     p.own_form = row_form(own_rows);
+    p.own_tiles = (int)((own_rows + form_rows(p.own_form) - 1) / form_rows(p.own_form));
+    // Few keys in all, or a short prefix in front of enough blocks: reading the prefix for every sequence (from L2) is
+    // cheaper than parts and a join behind them.
+    const long long own_blocks = (long long)batch * p.own_tiles * c.kv_heads;
+    p.front_steps = 0;
+    if (prefix_steps + own_steps <= 4 ||
+        (prefix_steps <= 4 && own_steps <= 16 && own_blocks >= (long long)form_blocks(c.head_dim, p.own_form) * sm_count())) {
+        p.front_steps = (int)prefix_steps;
+        p.tc_blocks = p.prefix_splits = p.prefix_tiles = 0;
+        p.prefix_form = p.own_form;
+        p.prefix_chunk = kTile;
+        p.own_splits = 1;
+        p.own_chunk = (int)std::max(1LL, own_steps) * kTile;
+        p.direct = true;
+        p.units = (size_t)rows * q_heads;
+        p.part_floats = 0;
+        return p;
+    }
+    const bool tc = prefix_rows > kTcRows && prefix_len > 0;
     p.prefix_form = row_form(prefix_rows);
     // one launch where the own keys are few (8 MB), in the prefix's form
     if (!tc && 4LL * batch * max_len * c.kv_heads * c.head_dim < (8LL << 20)) p.own_form = p.prefix_form;
     p.own_tiles = (int)((own_rows + form_rows(p.own_form) - 1) / form_rows(p.own_form));
     const int tile_rows = tc ? 2 * kTcTile : form_rows(p.prefix_form);
     p.prefix_tiles = (int)((prefix_rows + tile_rows - 1) / tile_rows);
-    const long long own_steps = (max_len + kTile - 1) / kTile, prefix_steps = (prefix_len + kTile - 1) / kTile;
     const long long total = c.kv_heads * (own_steps * batch * p.own_tiles + (tc ? 0 : prefix_steps * p.prefix_tiles));
     const long long fit = (long long)form_blocks(c.head_dim, p.own_form) * sm_count();
     const long long per = std::max(std::min(4LL, std::max(1LL, total / fit)), total / (kWaves * fit));
@@ -799,6 +838,7 @@ int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int 
     p.tc_blocks = plan.tc_blocks;
     p.behind_tc = 0;
     p.direct = plan.direct;
+    p.front_steps = plan.front_steps;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.err = device_error_word();
     if (!p.err) return fail(kBadHandle, "%s: no device error word", name);

@@ -32,6 +32,7 @@ struct AttendParams {
     int tc_blocks;      // > 0: the prefix is cut evenly over this many blocks of the tcgen05 kernel
     int behind_tc;      // the split kernel runs beside the tcgen05 kernel in front of it
     int direct;         // one slot in all: its kernel writes out itself
+    int front_steps;    // and this many steps over the prefix come in front of it
     float scale_log2;
     int *err;
 };

@@ -6,6 +6,7 @@ loader raises, telling the caller to build it (``python -m zillaphp_b200.build``
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -117,6 +118,11 @@ SIGNATURES: dict[str, tuple] = {
     "zilla_dp_detach": (I, [I]),
 }
 
+# Entry points of many integers that are called once a token: their argtypes stay unset, as ctypes passes plain ints by
+# itself in a third of the time that converting them through argtypes takes (0.8 us against 2.5 us for 15 arguments);
+# `call` below is the way to them.
+PLAIN_INTS = {"rope_dev", "zilla_kv_append", "zilla_kv_attend", "draft_verify_dev"}
+
 _lib: C.CDLL | None = None
 
 
@@ -133,9 +139,18 @@ def load() -> C.CDLL:
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = res
-        fn.argtypes = args
+        if name not in PLAIN_INTS:
+            fn.argtypes = args
     _lib = lib
     return lib
+
+
+def call(fn, *args) -> int:
+    """Calls a function of PLAIN_INTS; integers of other types (numpy's) are converted, anything else is refused."""
+    try:
+        return fn(*args)
+    except C.ArgumentError:
+        return fn(*[a if isinstance(a, C.c_float) else operator.index(a) for a in args])
 
 
 def last_error() -> str:
