@@ -58,9 +58,10 @@ struct PairSum {
 // Each warp sums one segment of the row; the segments' sums meet in the cluster's shared memory, and the
 // block that owns the crossing segment reads it again (it is in L2) to find the token.
 // Six blocks an SM (40 registers a thread), so that blocks that look for their row or for their token leave enough others
-// that stream: 29 us against 36 with four.
-template <bool VEC>
-__global__ void __launch_bounds__(kVerifyThreads, 6) draft_verify_kernel(const VerifyParams a) {
+// that stream: 29 us against 36 with four.  ALONE: so few blocks that no SM has a second one; then a thread's own loads
+// have to cover the latency, and four times as many are in flight (one row of 131,072: 7.9 against 7.2 us).
+template <bool VEC, bool ALONE>
+__global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_kernel(const VerifyParams a) {
     __shared__ double sums[kVerifyWarps];                      // read by the whole cluster
     __shared__ double all[kVerifyMaxCluster * kVerifyWarps];
     __shared__ double part[kVerifyWarps], s_base, s_target;
@@ -119,11 +120,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 6) draft_verify_kernel(const V
         const int begin = (int)min(lo, (long long)V), end = (int)min(lo + a.seg, (long long)V);
         PairSum sum;
         auto take = [&](int i, float x, float y) { sum.add(x, y, i != skip); };
-        // a batch of loads in front of its sums: 64 bytes a thread in flight
+        // a batch of loads in front of its sums: 64 bytes a thread in flight, or 256
         auto stream = [&](auto with_q) {
             constexpr bool kQ = decltype(with_q)::value;
             if constexpr (VEC) {
-                constexpr int kBatch = kQ ? 2 : 4;
+                constexpr int kBatch = (kQ ? 2 : 4) * (ALONE ? 4 : 1);
                 auto part4 = [&](int i, const float4 &x, const float4 &y) {
                     take(i, x.x, y.x);
                     take(i + 1, x.y, y.y);
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 6) draft_verify_kernel(const V
                     part4(i, *reinterpret_cast<const float4 *>(p + i), kQ ? *reinterpret_cast<const float4 *>(q + i) : zero);
                 for (; i < end; ++i) take(i, p[i], kQ ? q[i] : 0.0f);   // the row's last one to three elements, one lane's
             } else {
-                constexpr int kBatch = kQ ? 4 : 8;
+                constexpr int kBatch = (kQ ? 4 : 8) * (ALONE ? 4 : 1);
                 int i = begin + lane;
                 for (; i + 32 * (kBatch - 1) < end; i += 32 * kBatch) {
                     float x[kBatch], y[kBatch];
@@ -319,7 +320,8 @@ extern "C" int draft_verify_dev(int p_id, int p_ld, int q_id, int q_ld, int draf
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, vec ? draft_verify_kernel<true> : draft_verify_kernel<false>, a);
+    if (batch * ranks <= sm_count()) cudaLaunchKernelEx(&cfg, vec ? draft_verify_kernel<true, true> : draft_verify_kernel<false, true>, a);
+    else cudaLaunchKernelEx(&cfg, vec ? draft_verify_kernel<true, false> : draft_verify_kernel<false, false>, a);
     ZB_LAUNCH_CHECK(name);
     return kOk;
 }
