@@ -608,11 +608,12 @@ constexpr int kTcRows = 64;
 // Blocks of the tcgen05 kernel.  It takes whole SMs (one block each) and is bound by the tensor cores and the softmax, the own
 // keys' kernel behind it by HBM, and runs on the SMs that are left; so with n blocks the call takes about
 //   t = units / n * tile + start,  plus what the other SMs - n have not moved by then at the whole machine's rate,
-// and n minimises that.  Measured: a tile of 256 rows and 128 keys 2.4 us with head_dim 128, 2.1 below; an SM alone draws about
-// 85 GB/s, all together 5.8 TB/s.  Lengths are on the device: half of their bound is assumed.
+// and n minimises that.  Measured: a tile of 256 rows and 128 keys 1.9 us with head_dim 128, 1.75 below, and 12 us for the
+// start, the queries and the parts; an SM alone draws about 45 GB/s, all together 5.6 TB/s.  Lengths are on the device:
+// half of their bound is assumed.
 int choose_tc_blocks(const KvCache &c, long long units, double own_bytes) {
     const int sms = sm_count();
-    const double tile = c.head_dim == 128 ? 2.4e-6 : 2.1e-6, start = 6e-6, one = 85e9, all = 5.8e12;
+    const double tile = c.head_dim == 128 ? 1.9e-6 : 1.75e-6, start = 12e-6, one = 45e9, all = 5.6e12;
     int best = 1;
     double least = 1e30;
     for (int n = (int)std::min<long long>(units, sms); n >= 1 && n >= sms / 8; --n) {
