@@ -134,7 +134,10 @@ struct SplitRing {
     __device__ __forceinline__ bool wait(const AttendParams &p, int it) const {
         return __all_sync(0xffffffffu, wait_phase(full + it % ST, (it / ST) & 1, abort_flag, p.err, kErrFullWait)) != 0;
     }
-    __device__ __forceinline__ void done(int it) const {   // this warp has read the step's stage
+    // This warp has read the step's stage.  The fence orders its shared-memory reads before the copy (another proxy) that
+    // the arrival allows: without it a copy overtook reads still on their way, a handful of 16-wide columns in a run.
+    __device__ __forceinline__ void done(int it) const {
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + it % ST);
     }
