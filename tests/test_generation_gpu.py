@@ -555,3 +555,178 @@ def test_two_captured_calls_with_their_own_workspaces(bufs):
         n = loop.start[-1]
         assert torch.equal(bufs.get(loop.ids["out"], w.shape, torch.bfloat16)[:n], w[:n])
         loop.kv.close()
+
+
+# ---------------------------------------------------------------------------------------- refusals with real buffers
+def test_refusals_leave_everything_alone(bufs):
+    be, lib = bufs.be, native.load()
+    small, table, ints = bufs.new(3), bufs.new(34), bufs.put(i32([0, 1, 2, 0]))
+    x, y = bufs.put(torch.ones(2, 64)), bufs.put(torch.full((2, 64), 5.0))
+    be.ropeTableDev(table, 32)
+    kv = PagedKv(4, 16, 2, 32, "bf16")
+    other = PagedKv(4, 16, 2, 32, "fp16")
+
+    def rope(**kw):
+        a = {**dict(x=x, x_off=0, x_ld=64, y=y, y_off=0, y_ld=64, pos=ints, table=table, type=0, rows=2, heads=2, dim=32, rot=32, inter=0, inv=0), **kw}
+        return lib.rope_dev(*a.values())
+
+    for bad in (dict(x=small), dict(y=small), dict(rows=3), dict(pos=0), dict(table=small), dict(x_ld=66), dict(y_off=1, y_ld=65), dict(rot=34, dim=64, heads=1)):
+        assert rope(**bad) == -1, bad
+
+    def append(cache=kv, **kw):
+        a = {**dict(type=0, q=x, q_off=0, q_ld=64, k=x, k_off=0, k_ld=64, v=x, v_off=0, v_ld=64, qout=y, start=ints, len=ints, pages=ints, batch=2, rows=2,
+                    q_heads=2, max_pages=1, prefix=0, table=table, rot=32, inter=0), **kw}
+        return lib.zilla_kv_append(cache.id, *a.values())
+
+    for bad in (dict(q=small), dict(k=small), dict(v=small), dict(qout=small), dict(start=small, batch=3), dict(len=0), dict(pages=small, max_pages=2),
+                dict(rows=3), dict(table=small)):
+        assert append(**bad) == -1, bad
+    for bad in (dict(type=1 + 1), dict(type=3), dict(q_ld=63), dict(k_off=1), dict(v_off=-1), dict(q_heads=-1), dict(max_pages=0), dict(prefix=-1), dict(rot=34),
+                dict(rot=31), dict(qout=x), dict(k=kv.k_id), dict(v=kv.v_id), dict(qout=kv.k_id), dict(start=y), dict(inter=2), dict(prefix=2 ** 31 - 2)):
+        assert append(**bad) == -2, bad
+    assert append(cache=other, type=1) == -2           # rows of another 16-bit type than the cache's
+    assert append(q=small, q_heads=0, qout=0, len=bufs.put(i32([1, 1]))) == 0     # without queries theirs are not looked at
+
+    def attend(**kw):
+        a = {**dict(q=x, out=y, start=ints, len=ints, pages=ints, front=ints, batch=2, rows=2, heads=2, max_pages=1, prefix=0, max_new=1, max_len=16,
+                    scale=C.c_float(1.0), work=0), **kw}
+        return lib.zilla_kv_attend(kv.id, *a.values())
+
+    for bad in (dict(heads=3), dict(heads=0), dict(max_pages=0), dict(max_len=17), dict(max_new=0), dict(prefix=-1), dict(scale=C.c_float(math.inf)),
+                dict(scale=C.c_float(math.nan)), dict(out=x), dict(out=kv.k_id), dict(out=ints), dict(rows=2 ** 30, heads=4)):
+        assert attend(**bad) == -2, bad
+    for bad in (dict(q=small, rows=3), dict(out=small, heads=4), dict(start=small, batch=3), dict(len=0), dict(pages=small, max_pages=2), dict(prefix=100, front=small, rows=1, work=x),
+                dict(prefix=2000, front=bufs.new(125), work=small)):
+        assert attend(**bad) == -1, bad
+    assert attend(batch=0) == 0 and attend(rows=0, q=small, out=y) == 0
+
+    def verify(**kw):
+        a = {**dict(p=x, p_ld=64, q=0, q_ld=0, draft=ints, u=ints, start=ints, tokens=y, accepted=bufs.put(i32([9, 9])), batch=2, rows=2, vocab=64), **kw}
+        return lib.draft_verify_dev(*a.values())
+
+    for bad in (dict(p=small), dict(q=small, q_ld=64), dict(rows=3), dict(draft=0), dict(u=0), dict(start=small, batch=3), dict(tokens=0), dict(accepted=0), dict(vocab=65, p_ld=65)):
+        assert verify(**bad) == -1, bad
+    assert verify(batch=0) == 0
+    assert torch.equal(bufs.get(y, (2, 64), torch.float32), torch.full((2, 64), 5.0))
+    with pytest.raises(Exception, match="rope_dev failed"):
+        be.ropeDev(small, 0, 64, y, 0, 64, ints, table, 0, 2, 2, 32, 32)
+    with pytest.raises(Exception, match="zilla_kv_create failed"):
+        PagedKv(4, 17, 2, 32)
+    be.bufferFree(other.k_id)                           # a buffer taken away from a cache: the cache is refused, not read
+    assert lib.zilla_kv_k_id(other.id) == -1 and append(cache=other) == -1
+    other.close()
+    kv.close()
+
+
+def test_far_pages(bufs):
+    """A cache whose offsets pass 32 bits: its first, middle and last pages."""
+    pages, page, hk, dim, prefix = 140_000, 64, 4, 128, 200      # 4.6e9 elements of K, and of V
+    kv = PagedKv(pages, page, hk, dim, "bf16")
+    g = torch.Generator().manual_seed(31)
+    order = [pages - 1, 0, pages // 2, pages - 2, 1, 70_001, 139_000, 131_072]
+    front, own = i32(order[:4]), i32(order[4:]).reshape(2, 2)
+    x = torch.randn((prefix + 100, 2 * hk * dim), generator=g).to(torch.bfloat16)
+    i, shape = bufs.put(x), (prefix, hk, dim)
+    none = dict(table_id=0, rot_dim=0)
+    kv.append(1, 0, 0, 0, i, 0, 2 * hk * dim, i, hk * dim, 2 * hk * dim, 0, bufs.put(i32([0, prefix])), bufs.put(i32([prefix])), bufs.put(front), 1, prefix, 0, 4, 0, **none)
+    rest = bufs.put(x[prefix:])
+    start, length = [0, 70, 100], [70, 30]
+    kv.append(1, 0, 0, 0, rest, 0, 2 * hk * dim, rest, hk * dim, 2 * hk * dim, 0, bufs.put(i32(start)), bufs.put(i32(length)), bufs.put(own), 2, 100, 0, 2, prefix, **none)
+    q = torch.randn((5, 8, dim), generator=g).to(torch.bfloat16)
+    io = bufs.new(5 * 8 * dim)
+    work = kv.attend_work(2, 5, 8, prefix, 3, 70)
+    kv.attend(bufs.put(q), io, bufs.put(i32([0, 2, 5])), bufs.put(i32(length)), bufs.put(own), bufs.put(front), 2, 5, 8, 2, prefix, 3, 70, 0.1, bufs.new(max(1, work)))
+    got = bufs.get(io, (5, 8, dim), torch.bfloat16)
+    small = {n: k for k, n in enumerate(order)}
+    k, v = torch.zeros((8, hk, page, dim)).to(torch.bfloat16), torch.zeros((8, hk, page, dim)).to(torch.bfloat16)
+
+    def put(table, at, row):
+        k[small[int(table[at // page])], :, at % page] = x[row, : hk * dim].reshape(hk, dim)
+        v[small[int(table[at // page])], :, at % page] = x[row, hk * dim:].reshape(hk, dim)
+
+    for t in range(prefix):
+        put(front, t, t)
+    for b in range(2):
+        for t in range(length[b]):
+            put(own[b], t, prefix + start[b] + t)
+    ref = R.attend(q, k, v, [0, 2, 5], length, [[small[int(n)] for n in r] for r in own], [small[int(n)] for n in front], prefix, 0.1, page)
+    assert ((got.double() - ref[0]).abs() <= R.attend_tolerance(ref, dim, torch.bfloat16)).all()
+    kv.close()
+
+
+def test_calls_on_a_stream_of_the_program(bufs):
+    """The calls enqueued on torch's stream behind torch's own work, without a synchronisation between them."""
+    lib = native.load()
+    loop = Loop(bufs)
+    loop.new_step([4, 4, 4, 4, 4])
+    bufs.be.sync()
+    s = torch.cuda.Stream()
+    try:
+        lib.zilla_set_stream(C.c_void_p(s.cuda_stream))
+        with torch.cuda.stream(s):
+            a = torch.ones(4096, 4096, device="cuda")
+            for _ in range(20):
+                a = a @ a * 1e-4                  # the calls have to wait for this
+            loop.calls()
+        s.synchronize()
+    finally:
+        lib.zilla_set_stream(None)
+    loop.check()
+    loop.kv.close()
+
+
+# ---------------------------------------------------------------------------------------- autograd
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_autograd_rope(interleaved):
+    """A model that calls it: logits = rope(x W) read out, cross-entropy; the gradient of W against 64-bit differences of the
+    formula, and a shared leaf's gradients summed."""
+    from zillaphp_b200 import autograd as ag
+    g = np.random.default_rng(41)
+    rows, heads, dim, rot = 6, 2, 8, 6
+    x0, w0, u0 = g.standard_normal((rows, 5)), g.standard_normal((5, heads * dim)) * 0.4, g.standard_normal((heads * dim, 7)) * 0.4
+    pos, y = np.array([0, 1, 5, 70, 4000, -3]), np.array([0, 6, 3, 2, 1, 5])
+    plan = R.rates(rot, 10000.0, 3, 4.0, 64)
+
+    def loss64(w):
+        z = torch.from_numpy(x0 @ w).reshape(rows, heads, dim)
+        z, _ = R.rotate(z, torch.from_numpy(pos), rot, int(interleaved), plan)
+        z = z.reshape(rows, -1) @ torch.from_numpy(u0)
+        return float(torch.nn.functional.cross_entropy(z, torch.from_numpy(y)))
+
+    table = ag.RopeTable(rot, scaling="parts", factor=4.0, original=64)
+    w, u = ag.Parameter(w0), ag.Parameter(u0)
+    x = ag.Tensor.from_numpy(x0)
+
+    def forward():
+        z = x.matmul(w)
+        h = z.view((rows, heads, dim))
+        h._attach((z,), "view", lambda g_: z.accumulate_grad(g_.view(z.shape)))
+        r = h.rope(pos, table, interleaved)
+        flat = r.view((rows, heads * dim))
+        flat._attach((r,), "view", lambda g_: r.accumulate_grad(g_.view(r.shape)))
+        return ag.CrossEntropy()(flat.matmul(u), y)
+
+    loss = forward()
+    w64 = w.numpy().astype(np.float64)
+    assert abs(loss.item() - loss64(w64)) < 1e-5
+    loss.backward()
+    grad = w.grad.numpy().astype(np.float64)
+    # central differences in 64 bits: step 1e-4, their own error below step^2 times a third derivative of order 1; fp32: sums
+    # of a few dozen products of order 1, 2^-24 each
+    for i in range(5):
+        for j in range(heads * dim):
+            e = np.zeros_like(w64)
+            e[i, j] = 1e-4
+            d = (loss64(w64 + e) - loss64(w64 - e)) / 2e-4
+            assert abs(d - grad[i, j]) < 1e-5, (i, j, d, grad[i, j])
+    w.grad = None
+    a, b = forward(), forward()
+    a.backward()
+    b.backward()
+    assert np.max(np.abs(w.grad.numpy() - 2 * grad)) < 1e-5
+    with ag.no_grad():
+        z = ag.Tensor.from_numpy(np.ones((2, 1, 8))).rope([1, 2], table)
+        assert not z.requires_grad
+    for bad in ([1], [1.0, 2.0], [1, 2 ** 31]):
+        with pytest.raises(ValueError):
+            ag.Tensor.from_numpy(np.ones((2, 1, 8))).rope(bad, table)

@@ -23,6 +23,8 @@ Mirrors, with their semantics:
   Tensor::matmul     :1071-1089 matmul_dev; dA = g B^T (matmul_nt_dev), dB = A^T g (matmul_tn_dev)
   Tensor::relu       :1140-1154 relu_fwd_dev (mask) / relu_bwd_dev
   Tensor::noGrad     :54-62
+  rope               no counterpart: rotary positions of [..., heads, head_dim] (rope_dev; its gradient is
+                     the inverse turn, rope_dev with inverse = 1)
   CrossEntropy       src/Loss/CrossEntropy.php:18-85: the mean over the batch of
                      -log max(p_target, 1e-12) (:58); gradient (p - onehot) / B.
                      Computed by softmax_ce_clamped_dev in fp32 (the PHP class is
@@ -355,6 +357,45 @@ class Tensor:
                 b.accumulate_grad(gb)
 
         return out._attach((self, other), "mul", fn)
+
+
+    def rope(self, positions, table: "RopeTable", interleaved: bool = False) -> "Tensor":
+        """Rotary positions: the first table.rot_dim elements of every head of [..., heads, head_dim] turned at each
+        row's position (one int per row of heads), the rest copied."""
+        if len(self.shape) < 2:
+            raise ValueError(f"rope: [..., heads, head_dim] is needed, not {self.shape}.")
+        heads, dim = self.shape[-2:]
+        rows = self.size // (heads * dim)
+        at = np.ascontiguousarray(positions)
+        if at.size != rows or not np.issubdtype(at.dtype, np.integer):
+            raise ValueError(f"rope: {rows} integer positions are needed, not {at.size} of {at.dtype}.")
+        if rows and (at.min() < -2 ** 31 or at.max() >= 2 ** 31):
+            raise ValueError("rope: positions are 32-bit integers.")
+        be = backend()
+        pos = Tensor.from_numpy(at.astype(np.int32).view(np.float32).ravel())
+        out = Tensor.empty(self.shape)
+        x, wide, mode = self, heads * dim, int(bool(interleaved))
+        be.ropeDev(x.buf, 0, wide, out.buf, 0, wide, pos.buf, table.buf, 0, rows, heads, dim, table.rot_dim, mode, 0)
+
+        def fn(g: Tensor) -> None:
+            gi = Tensor.empty(x.shape)
+            be.ropeDev(g.buf, 0, wide, gi.buf, 0, wide, pos.buf, table.buf, 0, rows, heads, dim, table.rot_dim, mode, 1)
+            x.accumulate_grad(gi)
+
+        return out._attach((self,), "rope", fn)
+
+
+class RopeTable:
+    """The rotary frequencies of rot_dim elements (rope_table_dev): scaling "none", "linear", "base" or "parts"."""
+
+    SCALINGS = ("none", "linear", "base", "parts")
+
+    def __init__(self, rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 1,
+                 slow: float = 1.0, fast: float = 32.0):
+        self.rot_dim = rot_dim
+        self._held = Tensor.empty((rot_dim + 2,))
+        self.buf = self._held.buf
+        backend().ropeTableDev(self.buf, rot_dim, base, self.SCALINGS.index(scaling), factor, original, slow, fast)
 
 
 class Parameter(Tensor):

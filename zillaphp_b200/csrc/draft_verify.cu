@@ -272,8 +272,8 @@ extern "C" int draft_verify_dev(int p_id, int p_ld, int q_id, int q_ld, int draf
     if (p_ld < vocab || (q_id && q_ld < vocab)) return fail(kBadArg, "%s: a row stride is smaller than vocab", name);
     for (int to : {tokens_id, accepted_id})
         for (int from : {p_id, q_id, draft_id, u_id, start_id})
-            if (to == from) return fail(kBadArg, "%s: buffer %d is read and written", name, to);
-    if (tokens_id == accepted_id) return fail(kBadArg, "%s: tokens and accepted are one buffer", name);
+            if (to && to == from) return fail(kBadArg, "%s: buffer %d is read and written", name, to);
+    if (tokens_id && tokens_id == accepted_id) return fail(kBadArg, "%s: tokens and accepted are one buffer", name);
     const size_t n = rows;
     if (int rc = check_buffers(name, {{p_id, rows ? (n - 1) * p_ld + vocab : 0, "p"},
                                       {draft_id, n, "draft"},

@@ -1,6 +1,7 @@
 // kv_cache.cu -- the paged K/V cache: creation, and appending a batch's new
 // keys and values with the rotary rotation applied on the way.
 #include <map>
+#include <new>
 
 #include "kv_cache.cuh"
 #include "rope.cuh"
@@ -121,7 +122,8 @@ int zilla_kv_create(int pages, int page, int kv_heads, int head_dim, int type) {
     if (pages < 1 || kv_heads < 1 || kv_heads > 1024) return fail(kBadArg, "%s: bad sizes pages=%d kv_heads=%d", name, pages, kv_heads);
     const long long rows = (long long)pages * kv_heads * page;
     if (rows > 0x7fffffffLL - 128) return fail(kBadArg, "%s: %lld rows of keys are too many", name, rows);
-    KvCache *c = new KvCache();
+    KvCache *c = new (std::nothrow) KvCache();
+    if (!c) return fail(kBadHandle, "%s: out of host memory", name);
     c->pages = pages;
     c->page = page;
     while ((1 << c->page_log2) < page) ++c->page_log2;
@@ -138,6 +140,7 @@ int zilla_kv_create(int pages, int page, int kv_heads, int head_dim, int type) {
         c->v = ptr(c->v_id);
         cudaMemsetAsync(c->k, 0, floats * sizeof(float), stream());
         cudaMemsetAsync(c->v, 0, floats * sizeof(float), stream());
+        cudaStreamSynchronize(stream());   // zero before work on any other stream
         rc = check_cuda(name);
     }
     const uint64_t dims[2] = {(uint64_t)head_dim, (uint64_t)rows}, strides[1] = {(uint64_t)head_dim * 2};
@@ -146,14 +149,18 @@ int zilla_kv_create(int pages, int page, int kv_heads, int head_dim, int type) {
     const tc::Swizzle sw = head_dim < 64 ? tc::kSw64 : tc::kSw128;
     if (!rc) rc = tc::make_tmap_typed(&c->k_map, dtype, c->k, 2, dims, strides, box, sw);
     if (!rc) rc = tc::make_tmap_typed(&c->v_map, dtype, c->v, 2, dims, strides, box, sw);
-    if (rc) {
-        if (c->k_id > 0) zilla_buffer_free(c->k_id);
-        if (c->v_id > 0) zilla_buffer_free(c->v_id);
-        delete c;
-        return rc;
+    if (!rc) {
+        try {
+            g_caches[g_next_cache] = c;
+            return g_next_cache++;
+        } catch (...) {   // nothing is thrown through the C entry
+            rc = fail(kBadHandle, "%s: out of host memory", name);
+        }
     }
-    g_caches[g_next_cache] = c;
-    return g_next_cache++;
+    if (c->k_id > 0) zilla_buffer_free(c->k_id);
+    if (c->v_id > 0) zilla_buffer_free(c->v_id);
+    delete c;
+    return rc;
 }
 
 int zilla_kv_destroy(int kv) {
@@ -189,6 +196,7 @@ int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id,
         return fail(kBadArg, "%s: bad sizes batch=%d rows=%d q_heads=%d max_pages=%d prefix_len=%d", name, batch, rows,
                     q_heads, max_pages, prefix_len);
     const int D = c->head_dim;
+    if (interleaved != 0 && interleaved != 1) return fail(kBadArg, "%s: interleaved is 0 or 1", name);
     if ((long long)prefix_len + (long long)max_pages * c->page > 0x7fffffffLL)
         return fail(kBadArg, "%s: positions pass 31 bits", name);
     if (rot_dim < 0 || (rot_dim & 1) || rot_dim > D)

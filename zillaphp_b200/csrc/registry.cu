@@ -88,16 +88,16 @@ size_t capacity(int id) {
 }
 
 int check_buffers(const char *name, std::initializer_list<BufferNeed> needs) {
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess) return check_cuda(name);
     for (const BufferNeed &b : needs) {
         if (!ptr(b.id)) return fail(kBadHandle, "%s: invalid handle %d (%s)", name, b.id, b.what);
         if (g_slots[b.id].n < b.floats)
             return fail(kBadHandle, "%s: %s needs %zu floats, its buffer has %zu", name, b.what, b.floats, g_slots[b.id].n);
-        if (g_slots[b.id].device != dev)
-            return fail(kBadArg, "%s: %s is on device %d, the current device is %d", name, b.what,
-                        g_slots[b.id].device, dev);
     }
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return check_cuda(name);
+    for (const BufferNeed &b : needs)
+        if (g_slots[b.id].device != dev)
+            return fail(kBadArg, "%s: %s is on device %d, the current device is %d", name, b.what, g_slots[b.id].device, dev);
     return kOk;
 }
 

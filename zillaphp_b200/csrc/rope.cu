@@ -123,6 +123,8 @@ int rope_dev(int x_id, int x_off, int x_ld, int y_id, int y_off, int y_ld, int p
                     kRopeMaxDim);
     if (rot_dim < 2 || (rot_dim & 1) || rot_dim > head_dim)
         return fail(kBadArg, "%s: rot_dim %d is not an even number from 2 to head_dim", name, rot_dim);
+    if ((interleaved != 0 && interleaved != 1) || (inverse != 0 && inverse != 1))
+        return fail(kBadArg, "%s: interleaved and inverse are 0 or 1", name);
     const long long wide = (long long)heads * head_dim;
     if (wide > (1 << 24)) return fail(kBadArg, "%s: rows of %lld elements are too wide", name, wide);
     if (x_off < 0 || y_off < 0 || x_off + wide > x_ld || y_off + wide > y_ld)
