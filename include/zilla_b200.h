@@ -363,7 +363,8 @@ int zilla_lm_cache_length(int net);
 int rope_table_dev(int table_id, int rot_dim, float base, int scaling, float factor, int original, float slow,
                    float fast);
 /* Rotates the first rot_dim elements of every head of x [rows][heads][head_dim]
- * into y and copies the rest; row t at position pos[t] (any int32).  x_off, x_ld
+ * into y and copies the rest; row t at position pos[t] (any int32); the table is
+ * one of the same rot_dim.  x_off, x_ld
  * (and y_off, y_ld): the first head's offset in a row and the row stride, in
  * elements, so the queries of a packed projection are rotated where they lie.
  * interleaved 0: pairs (i, i + rot_dim / 2), 1: pairs (2i, 2i + 1).  inverse 1
@@ -424,7 +425,8 @@ long zilla_kv_attend_work(int kv, int batch, int rows, int q_heads, int prefix_l
  * tokens [rows]: the accepted drafts, the drawn token, then -1; accepted[b] = a.
  * Sums are fp64.  q_id 0: drafts made with certainty (q is one at the draft).
  * NaN and negative weights count as zero; u_k >= 1 takes the last token with a
- * weight; no weight at all gives token 0.  A draft outside the vocabulary fails. */
+ * weight; no weight at all gives token 0.  A draft outside the vocabulary fails
+ * (and is recorded, as are a sequence's rows that do not fit: accepted 0). */
 int draft_verify_dev(int p_id, int p_ld, int q_id, int q_ld, int draft_id, int u_id, int start_id, int tokens_id,
                      int accepted_id, int batch, int rows, int vocab);
 

@@ -126,6 +126,7 @@ def batch_of(new, length, prefix, page, seed, max_pages=0, spare=3):
     ([3], [70], 0, 2, 64, 64, 0, 32, 0, False, 0),                    # no queries
     ([2, 2], [9, 3], 2, 1, 32, 0, 0, 16, 0, True, 0),                 # no rotation
     ([2] * 300, [33] * 300, 2, 1, 32, 30, 0, 32, 3, False, 4),        # more sequences than threads
+    ([0, 1, 3, 0] * 700, [5] * 2800, 2, 1, 32, 32, 0, 16, 3, True, 3), # more than a block looks through one by one
 ])
 def test_append(bufs, src, dtype, new, length, hq, hk, dim, rot, interleaved, page, prefix, packed, pad):
     start, pages, _, count, most = batch_of(new, length, 0, page, 5)
@@ -247,6 +248,12 @@ def run_attend(bufs, dtype, new, length, hq, hk, dim, page, prefix, pad=0, max_n
 ])
 def test_attend(bufs, dtype, dim, new, length, hq, hk, page, prefix, pad):
     run_attend(bufs, dtype, new, length, hq, hk, dim, page, prefix, pad)
+
+
+def test_attend_large_batches(bufs):
+    """More sequences than a block of the join looks through one by one, empty ones among them."""
+    run_attend(bufs, "bf16", [0, 1, 0, 2] * 400, [i % 40 + 2 for i in range(1600)], 2, 1, 32, 16, 300, 3, only=list(range(0, 1600, 7)) + [1599])
+    run_attend(bufs, "fp16", [0] * 1200 + [3] + [0] * 1300, [3] * 2501, 4, 2, 64, 16, 700, 1)
 
 
 def test_attend_rows_without_keys(bufs):

@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kSplitThreads, kManyBlocks) attend_many_kernel
 template <typename T, int D, int BATCH>
 __global__ void __launch_bounds__(256, BATCH == 4 ? 5 : 2) attend_join_kernel(const __grid_constant__ AttendParams p) {
     constexpr int C = D / 32, kBatch = BATCH;
-    __shared__ int owner[8], own_slots[8];   // of the block's tokens, eight at most
+    __shared__ int owner[8], own_slots[8], range[2];   // of the block's tokens, eight at most
     griddep_launch();
     const int tid = threadIdx.x, lane = tid & 31;
     const long long unit0 = (long long)blockIdx.x * 8, units = (long long)p.batch.rows * p.q_heads, unit = unit0 + (tid >> 5);
@@ -538,8 +538,9 @@ __global__ void __launch_bounds__(256, BATCH == 4 ? 5 : 2) attend_join_kernel(co
         const int head = p.by_group.div(hq), row = t * p.group + hq - head * p.group;
         front = p.item_slots[head * p.prefix_tiles + row / (2 * kTcTile)];
     }
+    const int2 some = kv_range(range, p.batch.start, p.batch.batch, t0, n, tid, 256);
     __syncthreads();
-    for (int b = tid; b < p.batch.batch; b += 256) {   // every sequence looked at by one thread: no chain of dependent loads
+    for (int b = some.x + tid; b < some.y; b += 256) {
         const int first = p.batch.start[b], next = p.batch.start[b + 1], len = p.batch.len[b];
         const int lo = max(first, t0), hi = min(next, t0 + n);
         if (lo < hi && sequence_fits(p, first, next - first, len))
@@ -606,17 +607,17 @@ int form_rows(int form) { return form ? 8 * form : kManyRows; }
 int form_blocks(int head_dim, int form) { return form ? few_blocks(head_dim, form) : kManyBlocks; }
 
 // Rows that share the prefix's keys from which it goes to tcgen05.
-constexpr int kTcRows = 64;
+constexpr int kTcRows = 16;
 
 // Blocks of the tcgen05 kernel.  It takes whole SMs (one block each) and is bound by the tensor cores and the softmax, the own
 // keys' kernel behind it by HBM, and runs on the SMs that are left; so with n blocks the call takes about
 //   t = units / n * tile + start,  plus what the other SMs - n have not moved by then at the whole machine's rate,
-// and n minimises that.  Measured: a tile of 256 rows and 128 keys 1.9 us with head_dim 128, 1.75 below, and 12 us for the
-// start, the queries and the parts; an SM alone draws about 45 GB/s, all together 5.6 TB/s.  Lengths are on the device:
-// half of their bound is assumed.
+// and n minimises that.  Measured: a tile of 256 rows and 128 keys 2.2 us beside the other kernel with head_dim 128 (1.9
+// alone), 2.0 below, and 12 us for the start, the queries and the parts; an SM draws about 45 GB/s, all together 5.6 TB/s.
+// Lengths are on the device: half of their bound is assumed.
 int choose_tc_blocks(const KvCache &c, long long units, double own_bytes) {
     const int sms = sm_count();
-    const double tile = c.head_dim == 128 ? 1.9e-6 : 1.75e-6, start = 12e-6, one = 45e9, all = 5.6e12;
+    const double tile = c.head_dim == 128 ? 2.2e-6 : 2.0e-6, start = 12e-6, one = 45e9, all = 5.6e12;
     int best = 1;
     double least = 1e30;
     for (int n = (int)std::min<long long>(units, sms); n >= 1 && n >= sms / 8; --n) {
@@ -798,7 +799,8 @@ int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int 
     const size_t q_floats = elem_floats(plan.units * c->head_dim, c->type);
     if (int rc = check_buffers(name, {{q_id, q_floats, "q"},
                                       {out_id, q_floats, "out"},
-                                      {c->k_id, 0, "the cache"},
+                                      {c->k_id, c->floats, "the cache"},
+                                      {c->v_id, c->floats, "the cache"},
                                       {start_id, (size_t)batch + 1, "start"},
                                       {len_id, (size_t)batch, "len"},
                                       {pages_id, (size_t)batch * max_pages, "pages"}}))

@@ -29,7 +29,7 @@ struct AppendParams {
 // rows' sequences (a look at every start) and slots.
 template <typename TI, typename TO, int V, bool INTER>
 __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) kv_append_kernel(const AppendParams p) {
-    __shared__ int owner[kRopeThreads];
+    __shared__ int owner[kRopeThreads], range[2];
     griddep_launch();
     griddep_wait();
     const int u = threadIdx.x % p.shape.units, rest = threadIdx.x / p.shape.units, lane = rest % p.grid.lanes;
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) kv_append_kernel(co
     };
     int h0 = blockIdx.y * p.grid.lanes + lane;
     load(h0);
-    kv_owners(owner, p.batch.start, p.batch.batch, row0, n, threadIdx.x, blockDim.x);
+    kv_owners(owner, range, p.batch.start, p.batch.batch, row0, n, threadIdx.x, blockDim.x);
     const int b = works ? owner[in_block] : -1;
     if (b < 0) return;
     const int first = p.batch.start[b], own = p.batch.len[b] - (p.batch.start[b + 1] - first) + ((int)row - first), at = own >> p.page_log2;
@@ -131,7 +131,7 @@ int zilla_kv_create(int pages, int page, int kv_heads, int head_dim, int type) {
     c->head_dim = head_dim;
     c->type = type;
     c->box_rows = page < 64 ? page : 64;
-    const size_t floats = (size_t)rows * head_dim / 2;
+    const size_t floats = c->floats = (size_t)rows * head_dim / 2;
     c->k_id = zilla_buffer_alloc(floats);
     if (c->k_id > 0) c->v_id = zilla_buffer_alloc(floats);
     int rc = c->k_id > 0 && c->v_id > 0 ? kOk : kBadHandle;
@@ -216,7 +216,8 @@ int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id,
     };
     if (int rc = check_buffers(name, {{k_id, span(k_off, k_ld, wk), "k"},
                                       {v_id, span(v_off, v_ld, wk), "v"},
-                                      {c->k_id, 0, "the cache"},
+                                      {c->k_id, c->floats, "the cache"},
+                                      {c->v_id, c->floats, "the cache"},
                                       {start_id, (size_t)batch + 1, "start"},
                                       {len_id, (size_t)batch, "len"},
                                       {pages_id, (size_t)batch * max_pages, "pages"}}))

@@ -16,6 +16,7 @@ struct KvCache {
     void *k = nullptr, *v = nullptr;
     CUtensorMap k_map, v_map;   // [pages * kv_heads * page][head_dim], box {min(head_dim, 64), box_rows}
     int box_rows = 0;           // rows of one TMA box: a page, 64 at most
+    size_t floats = 0;          // registry floats of K, and of V
 };
 
 // The cache of an id; nullptr when unknown, or when one of its buffers was freed.
@@ -35,14 +36,38 @@ struct KvBatch {
     int batch, rows, max_pages, prefix_len;
 };
 
-// The sequences of the block's rows row0 .. row0 + n - 1 into owner[] (shared memory; -1 behind the
-// last sequence).  Every thread looks at batch / threads sequences, so there is no chain of dependent
-// loads as in a search.  Ends with the block synchronised.
-__device__ __forceinline__ void kv_owners(int *owner, const int *__restrict__ start, int batch, int row0, int n,
+// The sequences [first, last) that can own one of the rows row0 .. row0 + n - 1: all of a small batch; of a large one what
+// lies between two of 256 evenly spaced starts, so that a block looks at a few hundred sequences and not at all of them.
+// range: two ints of shared memory.  Ends with the block synchronised.
+__device__ __forceinline__ int2 kv_range(int *range, const int *__restrict__ start, int batch, int row0, int n, int tid, int threads) {
+    constexpr int kAll = 1024, kMarks = 256;
+    if (batch <= kAll) return make_int2(0, batch);
+    const int step = (batch + kMarks - 1) / kMarks;
+    if (tid == 0) {
+        range[0] = 0;
+        range[1] = batch;
+    }
+    __syncthreads();
+    for (int i = tid; i < kMarks; i += threads) {
+        const int b = i * step;
+        if (b >= batch) continue;
+        const int s = start[b];
+        if (s <= row0) atomicMax(range, b);
+        if (s >= row0 + n) atomicMin(range + 1, b);
+    }
+    __syncthreads();
+    return make_int2(range[0], range[1]);
+}
+
+// The sequences of the block's rows row0 .. row0 + n - 1 into owner[] (shared memory; -1 behind the last sequence).
+// Every thread looks at some of the sequences, so there is no chain of dependent loads as in a search.  Ends with the
+// block synchronised.
+__device__ __forceinline__ void kv_owners(int *owner, int *range, const int *__restrict__ start, int batch, int row0, int n,
                                           int tid, int threads) {
     for (int i = tid; i < n; i += threads) owner[i] = -1;
+    const int2 some = kv_range(range, start, batch, row0, n, tid, threads);
     __syncthreads();
-    for (int b = tid; b < batch; b += threads) {
+    for (int b = some.x + tid; b < some.y; b += threads) {
         const int lo = max(start[b], row0), hi = min(start[b + 1], row0 + n);
         for (int t = lo; t < hi; ++t) owner[t - row0] = b;
     }
