@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(256, BATCH == 4 ? 5 : 2) attend_join_kernel(co
     int front = p.prefix_splits;   // the prefix's slots come first
     if (p.tc_blocks && unit < units) {
         const int head = p.by_group.div(hq), row = t * p.group + hq - head * p.group;
-        front = p.item_slots[head * p.prefix_tiles + row / (2 * kTcTile)];
+        front = p.item_slots[row / (2 * kTcTile) * p.kv_heads + head];
     }
     const int2 some = kv_range(range, p.batch.start, p.batch.batch, t0, n, tid, 256);
     __syncthreads();
@@ -606,21 +606,25 @@ int row_form(long long rows) {
 int form_rows(int form) { return form ? 8 * form : kManyRows; }
 int form_blocks(int head_dim, int form) { return form ? few_blocks(head_dim, form) : kManyBlocks; }
 
-// Rows that share the prefix's keys from which it goes to tcgen05.
+// Up to as many rows share the prefix's keys in the mma.sync kernels, more on tcgen05, although they leave its 256-row tiles
+// mostly empty: 8 sequences of four query heads a key head behind 2029 keys 18.5 us against 20.4, behind 16000 keys 31 against
+// 46; two sequences behind 500 keys take the first form.
 constexpr int kTcRows = 16;
 
 // Blocks of the tcgen05 kernel.  It takes whole SMs (one block each) and is bound by the tensor cores and the softmax, the own
 // keys' kernel behind it by HBM, and runs on the SMs that are left; so with n blocks the call takes about
 //   t = units / n * tile + start,  plus what the other SMs - n have not moved by then at the whole machine's rate,
-// and n minimises that.  Measured: a tile of 256 rows and 128 keys 2.2 us beside the other kernel with head_dim 128 (1.9
-// alone), 2.0 below, and 12 us for the start, the queries and the parts; an SM draws about 45 GB/s, all together 5.6 TB/s.
-// Lengths are on the device: half of their bound is assumed.
-int choose_tc_blocks(const KvCache &c, long long units, double own_bytes) {
+// and the n that minimises it is taken, among the multiples of the row tiles where they are few.  Measured on the prefix
+// alone: a tile of 256 rows and 128 keys 2.2 us with head_dim 128, 1.8 with 64 (beside the own keys 2.8 to 3.7 and 1.7: both
+// kernels draw on L2 and HBM); 12 us stands for the start, the queries and the parts; an SM draws about 45 GB/s, all together 5.6 TB/s.  The choice is flat: 82 and 87 blocks take the same time within
+// the spread between runs.  Lengths are on the device: half of their bound is assumed.
+int choose_tc_blocks(const KvCache &c, int row_tiles, long long units, double own_bytes) {
     const int sms = sm_count();
-    const double tile = c.head_dim == 128 ? 2.2e-6 : 2.0e-6, start = 12e-6, one = 45e9, all = 5.6e12;
+    const double tile = c.head_dim == 128 ? 2.2e-6 : 1.8e-6, start = 12e-6, one = 45e9, all = 5.6e12;
     int best = 1;
     double least = 1e30;
-    for (int n = (int)std::min<long long>(units, sms); n >= 1 && n >= sms / 8; --n) {
+    const int step = row_tiles <= sms / 8 ? row_tiles : 1;
+    for (int n = (int)std::min<long long>(units, sms) / step * step; n >= 1 && n >= sms / 8; n -= step) {
         const double t = (double)((units + n - 1) / n) * tile + start, left = std::max(0.0, own_bytes - (sms - n) * one * t);
         if (t + left / all < least) {
             least = t + left / all;
@@ -675,7 +679,7 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
     p.tc_blocks = 0;
     if (tc) {
         const long long tiles = (prefix_len + kTcTile - 1) / kTcTile, units = tiles * c.kv_heads * p.prefix_tiles;
-        p.tc_blocks = choose_tc_blocks(c, units, 0.5 * 4.0 * batch * max_len * c.kv_heads * c.head_dim);
+        p.tc_blocks = choose_tc_blocks(c, p.prefix_tiles, units, 0.5 * 4.0 * batch * max_len * c.kv_heads * c.head_dim);
         const long long each = units / p.tc_blocks;   // a block's units at least
         p.prefix_splits = (int)std::min<long long>((tiles + each - 2) / each + 1, p.tc_blocks);
     }

@@ -87,8 +87,7 @@ __device__ __forceinline__ int box_row(const AttendParams &p, const int *pages, 
     return box_row_of(p, __ldcg(pages + (key >> p.page_log2)), kv_head, key);
 }
 
-// tc::mbar_wait with the clock read only after 64 failed tries: reading %globaltimer between the first two tries delays
-// nearly every wait of these kernels' handshakes by that read.
+// tc::mbar_wait with the clock read only after 64 failed tries: short waits do without it.
 __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort, int *err, int code) {
     uint64_t t0 = 0;
     for (uint32_t i = 1;; ++i) {

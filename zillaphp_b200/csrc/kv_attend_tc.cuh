@@ -2,20 +2,21 @@
 // (tokens x query heads of a kv head) fill 128-row tiles.
 //
 // An item is two 128-row tiles ("streams") of one kv head; both streams use each K and V tile of 128 keys, so a
-// tile crosses L2 once for 256 rows.  A block takes an even share of all items' key tiles (PrefixCut): parts of one to
-// a few items ("segments"), one after the other.  Per tile and stream:
-// in two steps of 64 keys:
+// tile crosses L2 once for 256 rows.  Items run over the heads first, then over the rows, and a block takes an even share of
+// all items' key tiles (PrefixCut): parts of one to a few items ("segments"), one after the other.  With a block count that
+// the row tiles divide, the blocks of all row tiles stand at the same keys at the same time and read them from HBM once
+// (128 sequences of 2 to 5 tokens, head_dim 128, 16384 shared keys and up to 2048 own: 217 to 225 us, 235 to 246 with the rows
+// first; 32768 shared keys 359 to 368, 382 to 392).  Per tile and stream, in two steps of 64 keys:
 //   S = Q K^T          M = 128 rows, N = 64 keys, K = head_dim, fp32 in TMEM
 //   P = 2^(S - ref)    one thread a row; P (16 bits) replaces S in TMEM, two keys a column
 //   O += P V           A = P from TMEM, B = V [key][d] (N-major), N = head_dim, K = 64 keys, fp32 in TMEM
 // A stream has two S buffers of 64 columns, so that S of the next step is there when P of this one is done: the softmax
-// never waits for an MMA of its own stream.  (One buffer of 128 keys makes softmax, P V and Q K^T a chain: 2.4 us a
-// tile against the 1.6 us of this form.)
+// never waits for an MMA of its own stream (one buffer of 128 keys makes softmax, P V and Q K^T a chain).
 // ref is the row's maximum as of its last change: it follows the true maximum only when that has passed it
 // by 2^8 (then O and l are rescaled), so that O rarely has to travel through registers; weights stay
 // below 2^8 and l and O carry the same factor, so the quotient does not change.
 // Warps 0-3 and 4-7 are the streams' softmax, warp 8 loads (TMA through the page list), warps 9 and 10 issue the streams'
-// MMAs (one warp for both waits for one stream's softmax while the other's step could run: PLACEHOLDER).
+// MMAs, so that a wait for one stream's softmax does not hold up the other's step.
 //
 // Order of a stream's MMAs: P V of step h, then Q K^T of step h + 2 over the same TMEM columns; one thread
 // issues both and the tensor pipe takes them in order.
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
     auto segments = [&](auto fn) {
         for (int unit = unit0; unit < unit1;) {
             const int item = unit / cut.tiles, tile0 = unit - item * cut.tiles, tiles = min(cut.tiles - tile0, unit1 - unit);
-            const int row0 = item % p.prefix_tiles * 2 * kTcTile;
+            const int row0 = item / p.kv_heads * 2 * kTcTile;
             if (!fn(item, row0, rows - row0 > kTcTile ? 2 : 1, tile0, tiles)) return;
             unit += tiles;
         }
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         bool ok = true;
         int i = 0;   // loads so far: K of a tile, then V
         segments([&](int item, int, int, int tile0, int tiles) {
-            const int head = item / p.prefix_tiles;
+            const int head = item % p.kv_heads;
             for (int x = 0; x < 2 * tiles; ++x, ++i) {
                 const int st = i % ST;
                 const int at = lane < all ? box_row(p, p.prefix_pages, head, (tile0 + (x >> 1)) * kTcTile + r0, p.batch.prefix_len) : 0;
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             }
             ++segment;
             // this warp's 32 rows; row = (token, query head of the kv head), unit its place in q and in the parts
-            const int head = item / p.prefix_tiles, warp_row = row0 + s * kTcTile + (warp & 3) * 32, row = warp_row + lane;
+            const int head = item % p.kv_heads, warp_row = row0 + s * kTcTile + (warp & 3) * 32, row = warp_row + lane;
             const int t = row < rows ? p.by_group.div(row) : 0, unit = t * p.q_heads + head * p.group + (row < rows ? row - t * p.group : 0);
             {
                 // Q, 16 bytes a lane along the rows.  With a negative scale the queries change their sign, so that the largest
