@@ -624,7 +624,8 @@ int choose_tc_blocks(const KvCache &c, int row_tiles, long long units, double ow
     int best = 1;
     double least = 1e30;
     const int step = row_tiles <= sms / 8 ? row_tiles : 1;
-    for (int n = (int)std::min<long long>(units, sms) / step * step; n >= 1 && n >= sms / 8; n -= step) {
+    const int most = (int)std::min<long long>(units, sms) / step * step;
+    for (int n = most; n >= 1 && n >= std::min(most, sms / 8); n -= step) {
         const double t = (double)((units + n - 1) / n) * tile + start, left = std::max(0.0, own_bytes - (sms - n) * one * t);
         if (t + left / all < least) {
             least = t + left / all;
