@@ -307,6 +307,23 @@ def test_attend_many_rows_scales(bufs):
         run_attend(bufs, "bf16", [2] * 20, [20] * 20, 8, 1, 64, 16, 700, scale=scale, sharp=sharp)
 
 
+@pytest.mark.parametrize("dtype,dim,hq,hk,page,prefix,new,longest", [
+    ("bf16", 128, 64, 8, 16, 1, [5] * 22, 300), ("fp16", 128, 64, 8, 64, 63, [5] * 22, 270),     # less than a step, less than a tile
+    ("bf16", 64, 128, 8, 32, 127, [4] * 20, 300), ("fp16", 64, 128, 8, 128, 129, [4] * 21, 400),   # about a tile
+    ("bf16", 32, 64, 16, 16, 257, [3, 0, 1] * 20, 500),                                            # rows that end in a first stream
+    ("fp16", 32, 256, 8, 64, 200, [1, 2] * 9, 600), ("bf16", 128, 17, 1, 64, 900, [2] * 13, 90),   # fewer tiles than blocks, an odd group
+    ("fp16", 128, 3, 1, 16, 8000, [6], 70), ("bf16", 64, 24, 3, 128, 4100, [1] * 3, 40)])          # 18 and 24 rows
+def test_attend_prefix_and_replies(bufs, dtype, dim, hq, hk, page, prefix, new, longest):
+    """Prefixes that are enough work for a kernel of their own beside the sequences' own keys."""
+    length = [max(n, longest - 61 * i % longest) for i, n in enumerate(new)]
+    run_attend(bufs, dtype, new, length, hq, hk, dim, page, prefix, 2)
+
+
+def test_attend_long_prefix_scales(bufs):
+    for scale, sharp in ((-0.2, 1.5), (0.0, 1.5), (0.4, 8.0)):
+        run_attend(bufs, "fp16", [2] * 20, [20] * 20, 16, 2, 64, 16, 2800, scale=scale, sharp=sharp)
+
+
 def test_attend_bad_numbers_are_recorded():
     """A page number outside the cache counts as keys and values of zero; a length beyond the call's leaves its rows alone."""
     b = R.Buffers(B200Backend())

@@ -606,10 +606,12 @@ int row_form(long long rows) {
 int form_rows(int form) { return form ? 8 * form : kManyRows; }
 int form_blocks(int head_dim, int form) { return form ? few_blocks(head_dim, form) : kManyBlocks; }
 
-// Up to as many rows share the prefix's keys in the mma.sync kernels, more on tcgen05, although they leave its 256-row tiles
-// mostly empty: 8 sequences of four query heads a key head behind 2029 keys 18.5 us against 20.4, behind 16000 keys 31 against
-// 46; two sequences behind 500 keys take the first form.
-constexpr int kTcRows = 16;
+// The shared prefix goes to tcgen05 where more than kTcRows rows share its keys, although 17 leave a 256-row tile mostly empty:
+// 8 sequences of four query heads a key head behind 2029 keys 18.5 us against 20.4 of the mma.sync kernels, behind 16000 keys
+// 31 against 46.  And where it is enough work for that kernel's longer start, counted in 64 x 64 tiles x head_dim: one key
+// head, 128 rows, head_dim 128 behind 1000 keys (4096) 12.6 us against 10.6, behind 2029 (8192) 13.5 against 13.8; eight key
+// heads, 24 rows behind 1000 keys (16384) 11.7 against 12.2; head_dim 64, 72 rows behind 1000 keys (16384) 9.9 against 9.4.
+constexpr int kTcRows = 16, kTcWork = 12288;
 
 // Blocks of the tcgen05 kernel.  It takes whole SMs (one block each) and is bound by the tensor cores and the softmax, the own
 // keys' kernel behind it by HBM, and runs on the SMs that are left; so with n blocks the call takes about
@@ -663,7 +665,8 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
         p.part_floats = 0;
         return p;
     }
-    const bool tc = prefix_rows > kTcRows && prefix_len > 0;
+    const bool tc = prefix_rows > kTcRows &&
+                    (prefix_rows + kManyRows - 1) / kManyRows * prefix_steps * c.kv_heads * c.head_dim > kTcWork;
     p.prefix_form = row_form(prefix_rows);
     // one launch where the own keys are few (8 MB), in the prefix's form
     if (!tc && 4LL * batch * max_len * c.kv_heads * c.head_dim < (8LL << 20)) p.own_form = p.prefix_form;
