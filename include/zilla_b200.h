@@ -394,7 +394,8 @@ int zilla_kv_v_id(int kv);
  * or the cache's type; *_off and *_ld: as rope_dev's, of each input (one packed
  * projection, or three buffers).  q_heads 0: no Q.  rot_dim 0: no rotation (no
  * table).  A prefix is filled by the same call: batch 1, its page list as pages,
- * prefix_len 0. */
+ * prefix_len 0.  Sequences may share pages that they only read; where two of them
+ * append to one place of a page, either may be kept. */
 int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id, int k_off, int k_ld, int v_id,
                     int v_off, int v_ld, int qout_id, int start_id, int len_id, int pages_id, int batch, int rows,
                     int q_heads, int max_pages, int prefix_len, int table_id, int rot_dim, int interleaved);
@@ -423,7 +424,7 @@ long zilla_kv_attend_work(int kv, int batch, int rows, int q_heads, int prefix_l
  * from max(p_a - q_a, 0) (from p_a where that is zero throughout), else from p_k:
  * the lowest t whose sum of weights up to t is above u_k times the whole sum.
  * tokens [rows]: the accepted drafts, the drawn token, then -1; accepted[b] = a.
- * Sums are fp64.  q_id 0: drafts made with certainty (q is one at the draft).
+ * Sums keep 46 bits or more.  q_id 0: drafts made with certainty (q is one at the draft).
  * NaN and negative weights count as zero; u_k >= 1 takes the last token with a
  * weight; no weight at all gives token 0.  A draft outside the vocabulary fails
  * (and is recorded, as are a sequence's rows that do not fit: accepted 0). */

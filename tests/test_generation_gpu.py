@@ -268,6 +268,12 @@ def test_attend_loose_bounds(bufs, dtype):
     run_attend(bufs, dtype, [1, 3], [20, 300], 8, 2, 128, 16, 100, 1, max_new=9, max_len=1000, max_pages=80)
 
 
+@pytest.mark.parametrize("max_new", [2 ** 31 - 1, 2 ** 30 + 1, 2 ** 26])
+def test_attend_largest_bound_of_new_rows(bufs, max_new):
+    """Row tiles are counted from the rows that are there, also where max_new times the group passes 31 bits."""
+    run_attend(bufs, "bf16", [3, 1, 40], [20, 300, 90], 64, 1, 32, 16, 100, 1, max_new=max_new)
+
+
 @pytest.mark.parametrize("dtype,dim,hq,hk,page,prefix,new,longest", [
     ("bf16", 32, 4, 4, 16, 96, [1] * 16, 32), ("fp16", 64, 8, 2, 16, 5, [2, 1, 0, 3], 64), ("bf16", 128, 24, 1, 128, 65, [1, 3], 100),
     ("fp16", 128, 4, 2, 32, 130, [4] * 230, 90),          # a prefix in front of many sequences' own keys

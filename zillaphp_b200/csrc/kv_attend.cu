@@ -644,6 +644,7 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
     constexpr int kWaves = 3;
     Plan p;
     const int group = q_heads / c.kv_heads;
+    max_new = std::min(max_new, std::max(rows, 1));   // a loose bound: no sequence has more rows than the call
     const long long own_rows = (long long)max_new * group, prefix_rows = (long long)rows * group;
     const long long own_steps = (max_len + kTile - 1) / kTile, prefix_steps = (prefix_len + kTile - 1) / kTile;
     p.own_form = row_form(own_rows);

@@ -94,8 +94,8 @@ struct RopeLane {
     }
 };
 
-// The widest vector (`widest`, 16 bytes of the input's type, or less: 4, 2, 1 elements) that divides a head's halves (interleaved: its rotated part), its copied rest and every
-// offset and row stride of the call.
+// The widest vector (`widest`: 16 bytes of the input's type; or less: 4, 2, 1 elements) that divides a head's halves
+// (interleaved: its rotated part), its copied rest and every offset and row stride of the call.
 inline int rope_vector(int widest, int head_dim, int rot, int interleaved, std::initializer_list<long long> also) {
     long long all = (long long)head_dim | (interleaved ? rot : rot / 2);
     for (long long a : also) all |= a;
