@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             // O through shared memory (over this warp's rows of Q, whose MMAs are done), so that whole lines are written
             constexpr int kCols = D >= 64 ? 32 : 16, kChunks = kCols / 4;
             uint32_t high[16];   // head_dim 32: two halves of 16 columns, as its Q leaves no more room
-            uint8_t *stage = base + s * kTileBytes + (warp & 3) * 32 * D * 2;
+            uint8_t *stage = base + s * kTileBytes + (warp & 3) * 32 * kRowBytes;   // its rows of the first block: no other warp writes there
             const size_t at = (size_t)slot * p.batch.rows * p.q_heads;
 #pragma unroll
             for (int c = 0; c < D / kCols; ++c) {
