@@ -616,10 +616,13 @@ constexpr int kTcRows = 16, kTcWork = 12288;
 // Blocks of the tcgen05 kernel.  It takes whole SMs (one block each) and is bound by the tensor cores and the softmax, the own
 // keys' kernel behind it by HBM, and runs on the SMs that are left; so with n blocks the call takes about
 //   t = units / n * tile + start,  plus what the other SMs - n have not moved by then at the whole machine's rate,
-// and the n that minimises it is taken, among the multiples of the row tiles where they are few.  Measured on the prefix
-// alone: a tile of 256 rows and 128 keys 2.2 us with head_dim 128, 1.8 with 64 (beside the own keys 2.8 to 3.7 and 1.7: both
-// kernels draw on L2 and HBM); 12 us stands for the start, the queries and the parts; an SM draws about 45 GB/s, all together 5.6 TB/s.  The choice is flat: 82 and 87 blocks take the same time within
-// the spread between runs.  Lengths are on the device: half of their bound is assumed.
+// and the n that minimises it is taken, among the multiples of the row tiles where they are few.  A tile of 256 rows and 128
+// keys takes 2.2 us with head_dim 128 in a loop of such calls, which runs into the power limit (1.7 at full clock: 88% of the
+// measured matrix rate), 1.8 with 64; 12 us stands for the start, the queries and the parts; an SM draws about 45 GB/s, all
+// together 5.6 TB/s.  Lengths are on the device: half of their bound is assumed.  128 sequences of up to 2048 keys behind
+// 16384 (n = 96) take 199 us at full clock, with 80 blocks 222, with 112 204; 32 sequences of up to 700 behind 2029 (n = 64)
+// 24.6, with 32 blocks 21.1, with 96 25.5 (the other kernel's own start, which this leaves out; with it that shape gains 3%
+// and 64 sequences behind 1000 keys lose 7%).
 int choose_tc_blocks(const KvCache &c, int row_tiles, long long units, double own_bytes) {
     const int sms = sm_count();
     const double tile = c.head_dim == 128 ? 2.2e-6 : 1.8e-6, start = 12e-6, one = 45e9, all = 5.6e12;

@@ -5,13 +5,16 @@
 // tile crosses L2 once for 256 rows.  Items run over the heads first, then over the rows, and a block takes an even share of
 // all items' key tiles (PrefixCut): parts of one to a few items ("segments"), one after the other.  With a block count that
 // the row tiles divide, the blocks of all row tiles stand at the same keys at the same time and read them from HBM once
-// (128 sequences of 2 to 5 tokens, head_dim 128, 16384 shared keys and up to 2048 own: 217 to 225 us, 235 to 246 with the rows
-// first; 32768 shared keys 359 to 368, 382 to 392).  Per tile and stream, in two steps of 64 keys:
+// (128 sequences of 2 to 5 tokens, head_dim 128, 16384 shared keys and up to 2048 own, in a loop: 217 to 225 us, 235 to 246 with
+// the rows first; 32768 shared keys 359 to 368, 382 to 392).  Per tile and stream, in two steps of 64 keys:
 //   S = Q K^T          M = 128 rows, N = 64 keys, K = head_dim, fp32 in TMEM
 //   P = 2^(S - ref)    one thread a row; P (16 bits) replaces S in TMEM, two keys a column
 //   O += P V           A = P from TMEM, B = V [key][d] (N-major), N = head_dim, K = 64 keys, fp32 in TMEM
 // A stream has two S buffers of 64 columns, so that S of the next step is there when P of this one is done: the softmax
-// never waits for an MMA of its own stream (one buffer of 128 keys makes softmax, P V and Q K^T a chain).
+// never waits for an MMA of its own stream.  One buffer of 128 keys makes softmax, P V and Q K^T a chain: 206 us against 199
+// at full clock for the large batch above, with each row's softmax shared by two warps and the streams issued in turn (260 if
+// both streams' MMAs are issued side by side, which keeps them in step).  That sharing alone changes nothing (200), nor does
+// a delay between the streams: a tile takes 1.7 us with head_dim 128, 88% of what the measured matrix rate would give.
 // ref is the row's maximum as of its last change: it follows the true maximum only when that has passed it
 // by 2^8 (then O and l are rescaled), so that O rarely has to travel through registers; weights stay
 // below 2^8 and l and O carry the same factor, so the quotient does not change.
