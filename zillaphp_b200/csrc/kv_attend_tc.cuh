@@ -1,5 +1,5 @@
-// kv_attend_tc.cuh -- the shared prefix's part of zilla_kv_attend on tcgen05, for batches whose rows
-// (tokens x query heads of a kv head) fill 128-row tiles.
+// kv_attend_tc.cuh -- the shared prefix's part of zilla_kv_attend on tcgen05, for batches with enough rows
+// (tokens x query heads of a kv head) and keys.
 //
 // An item is two 128-row tiles ("streams") of one kv head; both streams use each K and V tile of 128 keys, so a
 // tile crosses L2 once for 256 rows.  Items run over the heads first, then over the rows, and a block takes an even share of
