@@ -395,6 +395,14 @@ def test_verify(bufs, vocab, ld, certain):
         run_verify(bufs, p, None if certain else q, draft, u, new, vocab, 2)
 
 
+@pytest.mark.parametrize("vocab,ld,batch", [(517, 517, 1500), (2100, 2100, 950), (25000, 25003, 500), (9000, 9000, 160)])
+def test_verify_many_sequences(bufs, vocab, ld, batch):
+    """More sequences than the machine holds at once, and about as many."""
+    new = [(1, 2, 3, 0)[b % 4] for b in range(batch)]
+    p, q, draft, u = rows_of(new, vocab, ld, 21)
+    run_verify(bufs, p, q, draft, u, new, vocab, 1)
+
+
 def test_verify_borders(bufs):
     """Equal probabilities, numbers of 0 and next to 1, every draft taken, none taken, over 32 drafts."""
     new = [40, 40, 3]

@@ -293,12 +293,12 @@ int clusters_at_once(void (*kernel)(VerifyParams), bool vec, int ranks) {
 // against eight blocks to a sequence: 192 rows of 32,000 14.2 us (four blocks) against 16.4, 384 rows 24.5 (two) against
 // 31.4; 192 rows of 100,003 30.5 (four) against 29.6.  A block has 512 elements at least.
 int choose_ranks(void (*kernel)(VerifyParams), bool vec, int batch, int vocab) {
-    const int most = std::max(1, std::min(kVerifyMaxCluster, vocab / 512));
-    for (long long rounds = 1;; ++rounds) {
-        int ranks = most;
-        while (ranks > 0 && batch > rounds * clusters_at_once(kernel, vec, ranks)) --ranks;
-        if (ranks == most || (long long)ranks * 24576 >= vocab) return std::max(1, ranks);
-    }
+    const int most = std::max(1, std::min(kVerifyMaxCluster, vocab / 512)), least = std::min(most, (vocab + 24575) / 24576);
+    const int fit = clusters_at_once(kernel, vec, least);
+    const long long rounds = ((long long)batch + fit - 1) / fit;
+    int ranks = most;
+    while (ranks > least && batch > rounds * clusters_at_once(kernel, vec, ranks)) --ranks;
+    return ranks;
 }
 
 }  // namespace
