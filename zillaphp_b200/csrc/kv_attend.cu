@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(256, BATCH == 4 ? 5 : 2) attend_join_kernel(co
     int front = p.prefix_splits;   // the prefix's slots come first
     if (p.tc_blocks && unit < units) {
         const int head = p.by_group.div(hq), row = t * p.group + hq - head * p.group;
-        front = p.item_slots[row / (2 * kTcTile) * p.kv_heads + head];
+        front = noted_slots(p.item_slots[row / (2 * kTcTile) * p.kv_heads + head], p.prefix_splits);
     }
     const int2 some = kv_range(range, p.batch.start, p.batch.batch, t0, n, tid, 256);
     __syncthreads();

@@ -53,6 +53,10 @@ __host__ __device__ __forceinline__ PrefixCut prefix_cut(int prefix_len, int ite
     return c;
 }
 
+// The slots of an item as the tcgen05 kernel noted them.  Where one of its waits has run out the note is missing and the word
+// is whatever the workspace held; the join never reads more than the prefix's slots.
+__host__ __device__ __forceinline__ int noted_slots(int note, int prefix_splits) { return (unsigned)note <= (unsigned)prefix_splits ? note : prefix_splits; }
+
 // Keys that row j of a sequence sees of its own: clamped to 0 .. len.
 __device__ __forceinline__ int own_limit(int len, int n, int j) { return max(0, len - n + j + 1); }
 
