@@ -768,3 +768,27 @@ def test_autograd_rope(interleaved):
     for bad in ([1], [1.0, 2.0], [1, 2 ** 31]):
         with pytest.raises(ValueError):
             ag.Tensor.from_numpy(np.ones((2, 1, 8))).rope(bad, table)
+
+
+@pytest.mark.parametrize("prefix,length,bound", [(0, 2 ** 31 - 5000, 0), (2 ** 31 - 5000, 1, 1), (1000, 70, 2 ** 31 - 6000)])
+def test_attend_lengths_near_31_bits(bufs, prefix, length, bound):
+    """Lengths and bounds of lengths whose last slot's end passes 31 bits.  All keys are zero, so that every key weighs the same; the
+    tokens' pages are page 0, whose values are 0, but for the last 2^23 keys, whose values are 1."""
+    page, T, keys = 128, torch.bfloat16, prefix + length
+    kv = PagedKv(2, page, 1, 32, "bf16")
+    bufs.write(kv.v_id, torch.stack([torch.zeros(1, page, 32), torch.ones(1, page, 32)]).to(T))
+    ones = min(1 << 23, (keys - 1) // page * page // 2) // page * page      # whole pages at the end, a part of one more
+    table = torch.zeros(-(-max(length, bound) // page), dtype=torch.int32)
+    front = torch.zeros(max(1, -(-prefix // page)), dtype=torch.int32)
+    long_, n = (front, prefix) if prefix > length else (table, length)
+    last = -(-n // page)
+    long_[last - ones // page: last] = 1
+    light = n - (last * page - ones)                                          # keys of value 1
+    q, io = torch.ones((1, 1, 32)).to(T), bufs.put(torch.full((1, 1, 32), 7.0).to(T))
+    work = kv.attend_work(1, 1, 1, prefix, 1, bound or length)
+    kv.attend(bufs.put(q), io, bufs.put(i32([0, 1])), bufs.put(i32([length])), bufs.put(table), bufs.put(front), 1, 1, 1, table.numel(), prefix, 1,
+              bound or length, 1.0, bufs.new(max(1, work)))
+    got, want = bufs.get(io, (1, 1, 32), T).double(), light / keys
+    # counts up to 2^24 are exact in fp32; the joined sums round at most 2^-24 a slot (under 2000), the result once
+    assert ((got - want).abs() <= want * (2.0 ** -8 + 2000 * 2.0 ** -24)).all(), (got[0, 0, 0], want)
+    kv.close()

@@ -51,7 +51,7 @@ __device__ __forceinline__ SplitItem split_item(const AttendParams &p, int item,
     x.rows = x.n * p.group;
     x.begin = x.slot * chunk;
     const int last_j = p.by_group.div(max(0, min(x.rows - 1, x.row0 + tile_rows - 1)));
-    x.end = min(min(x.begin + chunk, x.len), x.shared ? x.len : own_limit(x.len, x.n, last_j));
+    x.end = slot_end(x.begin, chunk, x.shared ? x.len : own_limit(x.len, x.n, last_j));
     x.front = x.shared ? 0 : p.front_steps;
     x.empty = x.row0 >= x.rows || (x.begin >= x.end && !(p.direct && x.slot == 0));
     if (!x.shared) x.slot += p.prefix_splits;
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(256, BATCH == 4 ? 5 : 2) attend_join_kernel(co
         if (lo < hi && sequence_fits(p, first, next - first, len))
             for (int x = lo; x < hi; ++x) {
                 owner[x - t0] = b;
-                own_slots[x - t0] = (min(len, own_limit(len, next - first, x - first)) + p.own_chunk - 1) / p.own_chunk;
+                own_slots[x - t0] = slots_of(min(len, own_limit(len, next - first, x - first)), p.own_chunk);
             }
     }
     __syncthreads();
@@ -673,17 +673,18 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
                     (prefix_rows + kManyRows - 1) / kManyRows * prefix_steps * c.kv_heads * c.head_dim > kTcWork;
     p.prefix_form = row_form(prefix_rows);
     // one launch where the own keys are few (8 MB), in the prefix's form
-    if (!tc && 4LL * batch * max_len * c.kv_heads * c.head_dim < (8LL << 20)) p.own_form = p.prefix_form;
+    if (!tc && 4.0 * batch * max_len * c.kv_heads * c.head_dim < (double)(8 << 20)) p.own_form = p.prefix_form;
     p.own_tiles = (int)((own_rows + form_rows(p.own_form) - 1) / form_rows(p.own_form));
     const int tile_rows = tc ? 2 * kTcTile : form_rows(p.prefix_form);
     p.prefix_tiles = (int)((prefix_rows + tile_rows - 1) / tile_rows);
-    const long long total = c.kv_heads * (own_steps * batch * p.own_tiles + (tc ? 0 : prefix_steps * p.prefix_tiles));
-    const long long fit = (long long)form_blocks(c.head_dim, p.own_form) * sm_count();
-    const long long per = std::max(std::min(4LL, std::max(1LL, total / fit)), total / (kWaves * fit));
-    p.own_chunk = (int)std::min(per, std::max(1LL, own_steps)) * kTile;
-    p.own_splits = (int)((max_len + p.own_chunk - 1) / p.own_chunk);
-    p.prefix_chunk = (int)std::min(per, std::max(1LL, prefix_steps)) * kTile;
-    p.prefix_splits = (int)(((long long)prefix_len + p.prefix_chunk - 1) / p.prefix_chunk);
+    // (as doubles: loose bounds of many sequences pass 63 bits)
+    const double total = c.kv_heads * ((double)own_steps * batch * p.own_tiles + (tc ? 0.0 : (double)prefix_steps * p.prefix_tiles));
+    const double fit = (double)form_blocks(c.head_dim, p.own_form) * sm_count();
+    const double per = std::max(std::min(4.0, std::max(1.0, floor(total / fit))), floor(total / (kWaves * fit)));
+    p.own_chunk = (int)std::min(per, (double)std::max(1LL, own_steps)) * kTile;
+    p.own_splits = slots_of(max_len, p.own_chunk);
+    p.prefix_chunk = (int)std::min(per, (double)std::max(1LL, prefix_steps)) * kTile;
+    p.prefix_splits = slots_of(prefix_len, p.prefix_chunk);
     p.tc_blocks = 0;
     if (tc) {
         const long long tiles = (prefix_len + kTcTile - 1) / kTcTile, units = tiles * c.kv_heads * p.prefix_tiles;

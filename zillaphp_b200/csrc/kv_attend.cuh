@@ -57,6 +57,13 @@ __host__ __device__ __forceinline__ PrefixCut prefix_cut(int prefix_len, int ite
 // is whatever the workspace held; the join never reads more than the prefix's slots.
 __host__ __device__ __forceinline__ int noted_slots(int note, int prefix_splits) { return (unsigned)note <= (unsigned)prefix_splits ? note : prefix_splits; }
 
+// Slots of `chunk` keys that `keys` keys take, and the end of the slot that starts at `begin`, `len` at most.  keys + chunk
+// and begin + chunk may pass 31 bits.
+__host__ __device__ __forceinline__ int slots_of(int keys, int chunk) { return keys > 0 ? (keys - 1) / chunk + 1 : 0; }
+__host__ __device__ __forceinline__ int slot_end(int begin, int chunk, int len) {
+    return begin < len && chunk < len - begin ? begin + chunk : len;
+}
+
 // Keys that row j of a sequence sees of its own: clamped to 0 .. len.
 __device__ __forceinline__ int own_limit(int len, int n, int j) { return max(0, len - n + j + 1); }
 
