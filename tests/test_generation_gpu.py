@@ -792,3 +792,49 @@ def test_attend_lengths_near_31_bits(bufs, prefix, length, bound):
     # counts up to 2^24 are exact in fp32; the joined sums round at most 2^-24 a slot (under 2000), the result once
     assert ((got - want).abs() <= want * (2.0 ** -8 + 2000 * 2.0 ** -24)).all(), (got[0, 0, 0], want)
     kv.close()
+
+
+def run_attend_minus_infinity(bufs, dtype, new, length, hq, hk, dim, page, prefix, front_gone, own_gone):
+    """The first front_gone keys of the prefix and the first own_gone of each sequence (whole pages) score -inf for every
+    row; the others score about -100, far below any starting value.  The reference leaves those keys out."""
+    T = R.DT[dtype]
+    start, pages, front, count, most = batch_of(new, length, prefix, page, 51)
+    g = torch.Generator().manual_seed(52)
+    k, v = (torch.randn((count, hk, page, dim), generator=g).to(T) for _ in range(2))
+    q = torch.randn((start[-1], hq, dim), generator=g).to(T)
+    scale = 1 / math.sqrt(dim)
+    q[..., 0] = 1.0
+    q[..., 1] = 8.0
+    k[..., 1] = -100.0 / (8.0 * scale)
+    gone = torch.cat([front[: front_gone // page]] + [r[: own_gone // page] for r in pages]).long()
+    seen = k.clone()
+    seen[gone, :, :, 0] = -math.inf
+    kv = PagedKv(count, page, hk, dim, dtype)
+    bufs.write(kv.k_id, seen)
+    bufs.write(kv.v_id, v)
+    io = bufs.put(torch.full((start[-1], hq, dim), 7.0).to(T))
+    work = kv.attend_work(len(new), start[-1], hq, prefix, max(new), max(length))
+    kv.attend(bufs.put(q), io, bufs.put(i32(start)), bufs.put(i32(length)), bufs.put(pages), bufs.put(front), len(new), start[-1], hq, most, prefix,
+              max(new), max(length), scale, bufs.new(max(1, work)))
+    got = bufs.get(io, (start[-1], hq, dim), T)
+    ref = R.attend(q, k, v, start, [n - own_gone for n in length], [r[own_gone // page:] for r in pages.tolist()],
+                   front[front_gone // page:].tolist(), prefix - front_gone, scale, page)
+    err = (got.double() - ref[0]).abs()
+    tol = R.attend_tolerance(ref, dim, T)
+    assert (err <= tol).all(), float((err / tol).nan_to_num(math.inf).max())
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype,new,length,hq,hk,dim,page,prefix,front_gone,own_gone", [
+    ("bf16", [1] * 33, [9] * 33, 32, 8, 128, 64, 1000, 64, 0),       # the prefix on tcgen05: a step, a tile, all of a block's tiles
+    ("fp16", [1] * 33, [9] * 33, 32, 8, 128, 64, 1000, 128, 0),
+    ("bf16", [3] * 11, [40] * 11, 32, 4, 64, 16, 3000, 1600, 0),
+    ("fp16", [2] * 40, [3] * 40, 16, 8, 32, 16, 4000, 208, 0),
+    ("bf16", [4] * 30, [30] * 30, 16, 2, 128, 128, 2000, 1920, 0),
+    ("bf16", [1] * 33, [9] * 33, 32, 8, 128, 64, 1024, 1024, 0),     # nothing is left of the prefix
+    ("bf16", [2, 1], [300, 290], 4, 2, 64, 16, 400, 256, 128),        # the other kernels
+    ("fp16", [5, 30], [300, 290], 8, 1, 64, 32, 400, 64, 64),
+    ("bf16", [1, 2], [80, 90], 4, 2, 64, 16, 96, 64, 32),             # in one launch
+])
+def test_attend_keys_that_score_minus_infinity(bufs, dtype, new, length, hq, hk, dim, page, prefix, front_gone, own_gone):
+    run_attend_minus_infinity(bufs, dtype, new, length, hq, hk, dim, page, prefix, front_gone, own_gone)

@@ -17,13 +17,16 @@
 // a delay between the streams: a tile takes 1.7 us with head_dim 128, 88% of what the measured matrix rate would give.
 // ref is the row's maximum as of its last change: it follows the true maximum only when that has passed it
 // by 2^8 (then O and l are rescaled), so that O rarely has to travel through registers; weights stay
-// below 2^8 and l and O carry the same factor, so the quotient does not change.
+// below 2^8 and l and O carry the same factor, so the quotient does not change.  Before the first finite score (a key may
+// be infinite) it is the lowest number: weights of zero, and the first finite score sets it, however low.
 // Warps 0-3 and 4-7 are the streams' softmax, warp 8 loads (TMA through the page list), warps 9 and 10 issue the streams'
 // MMAs, so that a wait for one stream's softmax does not hold up the other's step.
 //
 // Order of a stream's MMAs: P V of step h, then Q K^T of step h + 2 over the same TMEM columns; one thread
 // issues both and the tensor pipe takes them in order.
 #pragma once
+
+#include <float.h>
 
 #include "kv_attend.cuh"
 
@@ -364,8 +367,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
 #pragma unroll
                     for (int i = 1; i < 16; ++i) top[c] = fmaxf(top[c], __uint_as_float(v[c >> 1][(c & 1) * 16 + i]));
                 }
-                float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
-                if (!(m > -INFINITY)) m = h ? ref : 0.0f;   // no key yet
+                const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl, -FLT_MAX);
                 if (h == 0) ref = m;
                 else if (__any_sync(0xffffffffu, m > ref + 8.0f)) {
                     // O with the step before in it: S of the next step is committed behind that, or the segment's last steps themselves
