@@ -838,3 +838,47 @@ def run_attend_minus_infinity(bufs, dtype, new, length, hq, hk, dim, page, prefi
 ])
 def test_attend_keys_that_score_minus_infinity(bufs, dtype, new, length, hq, hk, dim, page, prefix, front_gone, own_gone):
     run_attend_minus_infinity(bufs, dtype, new, length, hq, hk, dim, page, prefix, front_gone, own_gone)
+
+
+def border_row(g, vocab, side, with_q):
+    """A row p, q and a number u whose border is known exactly: one large weight and the rest near 2^-27, in multiples of 2^-62,
+    some weights behind token t (which comes soon after the large one) moved until the sum up to t is 2^-40 of the whole sum above (side 1) u times that, or below it
+    (side -1).  Returns p, q, u and the token that has to be drawn."""
+    p = g.integers((1 << 23) + (1 << 20), (1 << 24) - (1 << 20), vocab).astype(np.int64)      # units of 2^-50: 2^-27 to 2^-26
+    q = g.integers(0, 1 << 20, vocab).astype(np.int64) if with_q else np.zeros(vocab, np.int64)   # units of 2^-62
+    h = int(g.integers(0, vocab * 3 // 4))
+    p[h] = 3 << 48                                                         # 0.75
+    p[vocab - 1] = q[vocab - 1] = 0                                        # the draft that fails
+    c = np.cumsum((p << 12) - q)
+    big = 1 << 24
+    u = -(-int(c[h + 20]) * big // int(c[-1]))                             # a few tokens behind the large one
+    t = int(np.searchsorted(c.astype(np.float64), u / big * float(c[-1])))
+    d = int(c[t]) * big - u * int(c[-1]) - side * (int(c[-1]) >> 16)       # what the border is too high by, times 2^24
+    more = d // u >> 12                                                    # units of 2^-50 behind t
+    each, rest = divmod(abs(more), 64)
+    sign = 1 if more > 0 else -1
+    p[t + 1: t + 65] += sign * each
+    p[t + 1] += sign * rest
+    c = np.cumsum((p << 12) - q)
+    d = int(c[t]) * big - u * int(c[-1])
+    assert int(c[-1]) >> 17 < side * d < int(c[-1]) >> 15 and h < t and t + 65 < vocab and p[t + 1: t + 65].min() >= 1 << 23 and p[t + 1: t + 65].max() < 1 << 24
+    return (p * 2.0 ** -50).astype(np.float32), (q * 2.0 ** -62).astype(np.float32), np.float32(u / big), t if side > 0 else t + 1
+
+
+@pytest.mark.parametrize("with_q", [False, True])
+@pytest.mark.parametrize("vocab,ld,batch", [(1 << 22, 1 << 22, 4), (3_000_001, 3_000_001, 6), (300_000, 300_000, 8), (300_001, 300_001, 40), (300_001, 300_004, 40)])
+def test_verify_next_to_a_border(bufs, vocab, ld, batch, with_q):
+    """One large weight and many small ones: each sum has to be good to 2^-42, so that a border 2^-40 away is on its side."""
+    g = np.random.default_rng(vocab + batch)
+    n = 2 if with_q else 1
+    p, q, u, want = np.zeros((n * batch, ld), np.float32), np.zeros((n * batch, ld), np.float32), np.zeros(n * batch, np.float32), []
+    for b in range(batch):
+        p[n * b, :vocab], q[n * b, :vocab], u[n * b + n - 1], token = border_row(g, vocab, 1 if b % 2 else -1, with_q)
+        want += [token, -1][:n]
+    draft = np.full(n * batch, vocab - 1, np.int32)
+    it, ia = bufs.new(n * batch), bufs.new(batch)
+    ip, iq = bufs.put(torch.from_numpy(p)), bufs.put(torch.from_numpy(q)) if with_q else 0
+    bufs.be.draftVerifyDev(ip, ld, iq, ld, bufs.put(torch.from_numpy(draft)), bufs.put(torch.from_numpy(u)), bufs.put(i32(range(0, n * batch + 1, n))), it, ia,
+                           batch, n * batch, vocab)
+    assert bufs.get(it, (n * batch,), torch.int32).tolist() == want
+    assert bufs.get(ia, (batch,), torch.int32).tolist() == [0] * batch

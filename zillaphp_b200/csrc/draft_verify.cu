@@ -7,8 +7,8 @@
 //   w = max(p_a - q_a, 0) where a draft failed, p_a behind the last one;
 //   the token drawn is the lowest t with w_0 + ... + w_t > r (w_0 + ... + w_{V-1}), r = u_k.
 // fp32 sums over a large vocabulary are off by more than the distance between neighbouring borders, and would make
-// the token depend on how a row is split: differences are exact and sums are kept to 46 bits or more, a warp's
-// part of a row as pairs of fp32 numbers, everything else in fp64.
+// the token depend on how a row is split: differences are exact and sums are kept to 42 bits, eight weights as a pair of
+// fp32 numbers, everything else in fp64 (whose own roundings count from some 2^24 entries on: 39 bits at 2^28).
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -39,10 +39,14 @@ struct VerifyParams {
 // w_t of one element in fp64; NaN counts as 0.
 __device__ __forceinline__ double residual(float p, float q) { return p > q ? (double)fminf(p, FLT_MAX) - (double)q : 0.0; }
 
-// The sum of many residuals as an unevaluated sum hi + lo of fp32 numbers: the difference p - q = d + e is exact
+// The sum of up to kPairTerms residuals as an unevaluated sum hi + lo of fp32 numbers: the difference p - q = d + e is exact
 // (Dekker 1971, p > q >= 0; a negative q costs at most lo's rounding), hi + d = h + t too (Knuth's two-sum), and lo
 // takes e and t.  Eleven additions on the fp32 pipe; the same sum in fp64 is bound by two conversions an element (47 us
 // against 29 us for 192 rows of 100,003).
+// lo is a plain fp32 sum: behind n terms of sum S it is at most (n + 1) 2^-24 S, and each step rounds it and e + t, so that
+// hi + lo is off by (n^2 / 2 + 2 n + 1) 2^-48 S at most: 2^-42 S for the eight terms that go into an fp64 sum together.
+// (A pair over a lane's whole part of a row has no such bound: 34 bits were left of 2000 terms behind one of 0.75.)
+constexpr int kPairTerms = 8;
 struct PairSum {
     float hi = 0.0f, lo = 0.0f;
     __device__ __forceinline__ void add(float p, float q, bool keep) {
@@ -119,8 +123,13 @@ __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_ke
         auto w = [&](int i) { return i == skip ? 0.0 : residual(p[i], q ? q[i] : 0.0f); };
         const long long lo = (long long)(rank * kVerifyWarps + warp) * a.seg;
         const int begin = (int)min(lo, (long long)V), end = (int)min(lo + a.seg, (long long)V);
+        double s = 0.0;
         PairSum sum;
         auto take = [&](int i, float x, float y) { sum.add(x, y, i != skip); };
+        auto flush = [&] {
+            s += (double)sum.hi + (double)sum.lo;
+            sum = PairSum();
+        };
         // a batch of loads in front of its sums: 64 bytes a thread in flight, or 256
         auto stream = [&](auto with_q) {
             constexpr bool kQ = decltype(with_q)::value;
@@ -142,10 +151,15 @@ __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_ke
                         y[e] = kQ ? *reinterpret_cast<const float4 *>(q + i + 128 * e) : zero;
                     }
 #pragma unroll
-                    for (int e = 0; e < kBatch; ++e) part4(i + 128 * e, x[e], y[e]);
+                    for (int e = 0; e < kBatch; ++e) {
+                        part4(i + 128 * e, x[e], y[e]);
+                        if ((e + 1) % (kPairTerms / 4) == 0) flush();
+                    }
                 }
-                for (; i + 3 < end; i += 128)
+                for (; i + 3 < end; i += 128) {
                     part4(i, *reinterpret_cast<const float4 *>(p + i), kQ ? *reinterpret_cast<const float4 *>(q + i) : zero);
+                    flush();
+                }
                 for (; i < end; ++i) take(i, p[i], kQ ? q[i] : 0.0f);   // the row's last one to three elements, one lane's
             } else {
                 constexpr int kBatch = (kQ ? 4 : 8) * (ALONE ? 4 : 1);
@@ -158,14 +172,20 @@ __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_ke
                         y[e] = kQ ? q[i + 32 * e] : 0.0f;
                     }
 #pragma unroll
-                    for (int e = 0; e < kBatch; ++e) take(i + 32 * e, x[e], y[e]);
+                    for (int e = 0; e < kBatch; ++e) {
+                        take(i + 32 * e, x[e], y[e]);
+                        if ((e + 1) % kPairTerms == 0 || e == kBatch - 1) flush();
+                    }
                 }
-                for (; i < end; i += 32) take(i, p[i], kQ ? q[i] : 0.0f);
+                for (int n = 1; i < end; i += 32, ++n) {
+                    take(i, p[i], kQ ? q[i] : 0.0f);
+                    if (n % kPairTerms == 0) flush();
+                }
             }
+            flush();
         };
         if (q) stream(std::true_type());
         else stream(std::false_type());
-        double s = (double)sum.hi + (double)sum.lo;
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) sums[warp] = s;
