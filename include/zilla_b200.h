@@ -424,11 +424,12 @@ long zilla_kv_attend_work(int kv, int batch, int rows, int q_heads, int prefix_l
  * from max(p_a - q_a, 0) (from p_a where that is zero throughout), else from p_k:
  * the lowest t whose sum of weights up to t is above u_k times the whole sum.
  * tokens [rows]: the accepted drafts, the drawn token, then -1; accepted[b] = a.
- * Sums are good to 2^-42 of themselves (2^-39 at the largest vocab, 2^28).  q_id 0: drafts made with certainty (q is one at
- * the draft).
- * NaN and negative weights count as zero; u_k >= 1 takes the last token with a
- * weight; no weight at all gives token 0.  A draft outside the vocabulary fails
- * (and is recorded, as are a sequence's rows that do not fit: accepted 0). */
+ * Sums are good to 2^-42 of themselves (2^-39 at the largest vocab, 2^28).
+ * q_id 0: drafts made with certainty (q is one at the draft).  NaN and negative
+ * weights count as zero, infinite p and q as the largest finite number; u_k >= 1
+ * takes the last token with a weight; no weight at all gives token 0.  A draft
+ * outside the vocabulary fails (and is recorded, as are a sequence's rows that do
+ * not fit: accepted 0). */
 int draft_verify_dev(int p_id, int p_ld, int q_id, int q_ld, int draft_id, int u_id, int start_id, int tokens_id,
                      int accepted_id, int batch, int rows, int vocab);
 

@@ -882,3 +882,29 @@ def test_verify_next_to_a_border(bufs, vocab, ld, batch, with_q):
                            batch, n * batch, vocab)
     assert bufs.get(it, (n * batch,), torch.int32).tolist() == want
     assert bufs.get(ia, (batch,), torch.int32).tolist() == [0] * batch
+
+
+@pytest.mark.parametrize("vocab,ld", [(700, 700), (701, 701), (100_003, 100_004), (100_003, 100_003)])
+@pytest.mark.parametrize("batch", [1, 160])
+def test_verify_largest_weights(bufs, vocab, ld, batch):
+    """Infinite weights count as the largest finite number; several of those in one thread's elements, alone and as residuals."""
+    top, inf, g = np.finfo(np.float32).max, np.float32(np.inf), np.random.default_rng(71)
+    p, q = np.zeros((3 * batch, ld), np.float32), np.zeros((3 * batch, ld), np.float32)
+    p[:, :vocab] = g.random((3 * batch, vocab), np.float32)
+    q[:, :vocab] = g.random((3 * batch, vocab), np.float32)
+    u, draft, new = g.random(3 * batch).astype(np.float32), np.full(3 * batch, 3, np.int32), [2, 1] * batch
+    p[0::3, 3] = 0.0                                                         # the draft fails: residuals
+    p[:, [4, 5, 6, 7, 36, 37, 68, 132, 133, 260]] = top
+    p[:, [5, 37, 640]] = inf
+    p[:, 641] = top / 1000                                                   # finite weights keep their proportions
+    q[:, [36, 68]] = top                                                     # no residual there
+    q[:, 132] = -top                                                         # twice the largest number
+    q[:, 6] = inf
+    finite = np.minimum(p, top)
+    start = starts(new)
+    it, ia = bufs.new(3 * batch), bufs.new(2 * batch)
+    bufs.be.draftVerifyDev(bufs.put(torch.from_numpy(p)), ld, bufs.put(torch.from_numpy(q)), ld, bufs.put(torch.from_numpy(draft)),
+                           bufs.put(torch.from_numpy(u)), bufs.put(i32(start)), it, ia, 2 * batch, 3 * batch, vocab)
+    tokens, accepted = R.verify(finite, q, draft, u, start, vocab)
+    assert bufs.get(it, (3 * batch,), torch.int32).tolist() == [tokens[i] for i in range(3 * batch)]
+    assert bufs.get(ia, (2 * batch,), torch.int32).tolist() == accepted

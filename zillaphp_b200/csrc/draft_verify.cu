@@ -36,8 +36,10 @@ struct VerifyParams {
     int *err;
 };
 
-// w_t of one element in fp64; NaN counts as 0.
-__device__ __forceinline__ double residual(float p, float q) { return p > q ? (double)fminf(p, FLT_MAX) - (double)q : 0.0; }
+// w_t of one element in fp64; NaN counts as 0, an infinity as the largest finite number.
+__device__ __forceinline__ double residual(float p, float q) {
+    return p > q ? (double)fminf(p, FLT_MAX) - (double)fmaxf(q, -FLT_MAX) : 0.0;
+}
 
 // The sum of up to kPairTerms residuals as an unevaluated sum hi + lo of fp32 numbers: the difference p - q = d + e is exact
 // (Dekker 1971, p > q >= 0; a negative q costs at most lo's rounding), hi + d = h + t too (Knuth's two-sum), and lo
@@ -58,6 +60,16 @@ struct PairSum {
         lo += e + t;
     }
 };
+
+// A warp's sum in fp64 throughout, for weights near the end of fp32's range.  Not inlined: its registers stay out of the kernel.
+__device__ __noinline__ double wide_sum(const float *p, const float *q, int skip, int begin, int end, int lane) {
+    double s = 0.0;
+    for (int i = begin + lane; i < end; i += 32)
+        if (i != skip) s += residual(p[i], q ? q[i] : 0.0f);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
 
 // Bound by HBM: one row of p, and one of q where a draft failed, read once by the sequence's cluster.
 // Each warp sums one segment of the row; the segments' sums meet in the cluster's shared memory, and the
@@ -188,6 +200,7 @@ __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_ke
         else stream(std::false_type());
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (!(s < INFINITY)) s = wide_sum(p, q, skip, begin, end, lane);   // a pair has passed fp32's range
         if (lane == 0) sums[warp] = s;
         cluster.sync();
         for (int i = tid; i < kVerifyMaxCluster * kVerifyWarps; i += kVerifyThreads)
