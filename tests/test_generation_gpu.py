@@ -908,3 +908,30 @@ def test_verify_largest_weights(bufs, vocab, ld, batch):
     tokens, accepted = R.verify(finite, q, draft, u, start, vocab)
     assert bufs.get(it, (3 * batch,), torch.int32).tolist() == [tokens[i] for i in range(3 * batch)]
     assert bufs.get(ia, (2 * batch,), torch.int32).tolist() == accepted
+
+
+@pytest.mark.parametrize("hq,hk,dim,prefix,new", [(4, 2, 64, 300, [1, 1, 2]), (4, 2, 64, 100, [1, 1, 2]), (64, 2, 128, 3000, [2, 1, 2]), (96, 1, 64, 4100, [1, 1, 1])])
+def test_attend_no_own_keys_at_all(bufs, hq, hk, dim, prefix, new):
+    """max_len 0: every row sees the prefix alone, and a sequence with a length all the same is recorded and left as it is."""
+    lib, page, T = native.load(), 16, torch.bfloat16
+    start, pages, front, count, most = batch_of(new, [0] * 3, prefix, page, 61)
+    g = torch.Generator().manual_seed(62)
+    k, v = (torch.randn((count, hk, page, dim), generator=g).to(T) for _ in range(2))
+    q = torch.randn((start[-1], hq, dim), generator=g).to(T)
+    kv = PagedKv(count, page, hk, dim, "bf16")
+    bufs.write(kv.k_id, k)
+    bufs.write(kv.v_id, v)
+    before = torch.full((start[-1], hq, dim), 7.0).to(T)
+    iq, it, ip, front_id = bufs.put(q), bufs.put(i32(start)), bufs.put(pages), bufs.put(front)
+    work = bufs.new(max(1, kv.attend_work(3, start[-1], hq, prefix, max(new), 0)))
+    ref = R.attend(q, k, v, start, [0] * 3, pages.tolist(), front.tolist(), prefix, 0.1, page)
+    tol = R.attend_tolerance(ref, dim, T)
+    for length in ([0, 0, 0], [0, 5, 0]):
+        io = bufs.put(before)
+        kv.attend(iq, io, it, bufs.put(i32(length)), ip, front_id, 3, start[-1], hq, most, prefix, max(new), 0, 0.1, work)
+        got = bufs.get(io, before.shape, T)
+        ok = torch.tensor([length[b] == 0 for b in range(3) for _ in range(new[b])])
+        assert ((got.double() - ref[0]).abs() <= tol)[ok].all()
+        assert torch.equal(got[~ok], before[~ok])
+        assert lib.zilla_check_device() == (-3 if any(length) else 0)
+    kv.close()

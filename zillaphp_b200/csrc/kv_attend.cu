@@ -682,7 +682,7 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
     const double fit = (double)form_blocks(c.head_dim, p.own_form) * sm_count();
     const double per = std::max(std::min(4.0, std::max(1.0, floor(total / fit))), floor(total / (kWaves * fit)));
     p.own_chunk = (int)std::min(per, (double)std::max(1LL, own_steps)) * kTile;
-    p.own_splits = slots_of(max_len, p.own_chunk);
+    p.own_splits = std::max(1, slots_of(max_len, p.own_chunk));   // one without own keys too: its blocks look at every sequence's sizes
     p.prefix_chunk = (int)std::min(per, (double)std::max(1LL, prefix_steps)) * kTile;
     p.prefix_splits = slots_of(prefix_len, p.prefix_chunk);
     p.tc_blocks = 0;
@@ -692,7 +692,6 @@ Plan make_plan(const KvCache &c, int batch, int rows, int q_heads, int prefix_le
         const long long each = units / p.tc_blocks;   // a block's units at least
         p.prefix_splits = (int)std::min<long long>((tiles + each - 2) / each + 1, p.tc_blocks);
     }
-    if (p.own_splits + p.prefix_splits == 0) p.own_splits = 1;   // no keys at all: the rows are still written
     p.direct = p.own_splits == 1 && p.prefix_splits == 0;
     p.units = (size_t)rows * q_heads;
     p.part_floats = p.direct ? 0 : p.units * (p.own_splits + p.prefix_splits) * (c.head_dim + 2);
