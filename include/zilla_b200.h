@@ -387,7 +387,10 @@ int zilla_kv_v_id(int kv);
  * the cache, the new ones included; its i-th own token lies in page
  * pages[b * max_pages + i / page].  Every sequence stands behind the same
  * prefix_len tokens (0: none), which lie in the pages of prefix_pages.  Rows
- * behind the last sequence (start[batch] .. rows - 1) are left as they are.
+ * behind the last sequence (start[batch] .. rows - 1) are left as they are.  A
+ * sequence with rows outside 0 .. rows - 1 is recorded and its rows are skipped;
+ * a start that is below the one before it may cost other sequences theirs.  With
+ * batch or rows 0 nothing is done.
  *
  * Appends the new rows' K and V, K rotated at position prefix_len + i, and writes
  * the rotated Q to qout [rows][q_heads][head_dim] of the cache's type.  x_type: 0

@@ -935,3 +935,34 @@ def test_attend_no_own_keys_at_all(bufs, hq, hk, dim, prefix, new):
         assert torch.equal(got[~ok], before[~ok])
         assert lib.zilla_check_device() == (-3 if any(length) else 0)
     kv.close()
+
+
+@pytest.mark.parametrize("spare", [0, 2000])
+@pytest.mark.parametrize("start,bad", [
+    ([0, 2, 9], [1]), ([0, 2, 4, 6], [2]), ([0, 2, 4, 9, 12], [2, 3]), ([-1, 1, 3], [0]), ([0, 2, 2 ** 31 - 1], [1]), ([-2 ** 31, 2, 4], [0]),
+    ([0, 2, 1, 1], [1]), ([0, 3, -5], [1])])
+def test_append_rows_that_do_not_fit_are_recorded(bufs, start, bad, spare):
+    """A sequence with rows outside the call's four, or with fewer than none, is recorded and none of its rows is stored; the
+    others are.  Alone, and in front of many empty sequences; there, a start that steps back may cost the others their rows too
+    (which are found between starts that rise), but stores nothing wrong."""
+    lib, T = native.load(), torch.bfloat16
+    size, rows = len(start) - 1, 4
+    kv = PagedKv(size + 1, 16, 1, 32, "bf16")
+    shape = (size + 1, 1, 16, 32)
+    want_k = torch.full(shape, 3.0).to(T)
+    bufs.write(kv.k_id, want_k)
+    bufs.write(kv.v_id, want_k)
+    x, want = torch.arange(1, rows + 1).float()[:, None].expand(rows, 32).contiguous(), torch.full((rows, 1, 32), 7.0).to(T)
+    ix, io, total = bufs.put(x), bufs.put(want), size + spare
+    kv.append(0, ix, 0, 32, ix, 0, 32, ix, 0, 32, io, bufs.put(i32(start + [start[-1]] * spare)), bufs.put(i32([16] * total)),
+              bufs.put(i32([[min(b, size)] for b in range(total)])), total, rows, 1, 1, 0, 0, 0)
+    for b in range(size):
+        for t in range(start[b], start[b + 1]) if b not in bad else ():
+            want[t] = x[t].to(T)
+            want_k[b, :, 16 - start[b + 1] + t] = x[t].to(T)
+    assert lib.zilla_check_device() == -3 and lib.zilla_check_device() == 0
+    got, got_k, got_v = bufs.get(io, want.shape, T), bufs.get(kv.k_id, shape, T), bufs.get(kv.v_id, shape, T)
+    if spare and any(start[b] > start[b + 1] for b in range(size)):
+        want, want_k = torch.where(got == 7.0, got, want), torch.where(got_k == 3.0, got_k, want_k)
+    assert torch.equal(got, want) and torch.equal(got_k, want_k) and torch.equal(got_v, want_k)
+    kv.close()

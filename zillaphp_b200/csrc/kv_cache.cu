@@ -12,6 +12,8 @@ namespace {
 std::map<int, KvCache *> g_caches;
 int g_next_cache = 1;
 
+constexpr int kCheckBatch = 1024;
+
 struct AppendParams {
     const void *q, *k, *v;
     void *q_out, *k_cache, *v_cache;
@@ -21,6 +23,7 @@ struct AppendParams {
     int q_heads, kv_heads, page_log2, pages;
     RopeShape shape;
     RopeGrid grid;   // over the q, k and v heads together
+    unsigned row_blocks;   // blocks along x that take rows; the ones behind them check kCheckBatch sequences each
     int *err;
 };
 
@@ -32,6 +35,14 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) kv_append_kernel(co
     __shared__ int owner[kRopeThreads], range[2];
     griddep_launch();
     griddep_wait();
+    // Blocks that only check: a sequence outside the call's rows may be seen by none that takes rows.  Checked by those, in
+    // their look at the starts, it costs 2% of a prompt's time; so, one more block, 0.1 us of a call.
+    if (blockIdx.x >= p.row_blocks) {
+        const int b0 = (blockIdx.x - p.row_blocks) * kCheckBatch, b1 = b0 + min(kCheckBatch, p.batch.batch - b0);
+        for (int b = b0 + threadIdx.x; b < b1 && blockIdx.y == 0; b += blockDim.x)
+            if (!kv_rows_fit(p.batch, p.batch.start[b], p.batch.start[b + 1])) atomicCAS(p.err, 0, kErrKvLength);
+        return;
+    }
     const int u = threadIdx.x % p.shape.units, rest = threadIdx.x / p.shape.units, lane = rest % p.grid.lanes;
     const int in_block = rest / p.grid.lanes, row0 = blockIdx.x * p.grid.rows, n = min(p.grid.rows, p.batch.rows - row0);
     const bool works = in_block < n;
@@ -52,7 +63,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) kv_append_kernel(co
     };
     int h0 = blockIdx.y * p.grid.lanes + lane;
     load(h0);
-    kv_owners(owner, range, p.batch.start, p.batch.batch, row0, n, threadIdx.x, blockDim.x);
+    kv_owners(owner, range, p.batch, row0, n, threadIdx.x, blockDim.x);
     const int b = works ? owner[in_block] : -1;
     if (b < 0) return;
     const int first = p.batch.start[b], own = p.batch.len[b] - (p.batch.start[b + 1] - first) + ((int)row - first), at = own >> p.page_log2;
@@ -86,7 +97,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) kv_append_kernel(co
 
 template <typename TI, typename TO, bool INTER>
 void launch_append(const AppendParams &p, int vec) {
-    const dim3 grid((unsigned)((p.batch.rows + (long long)p.grid.rows - 1) / p.grid.rows), p.grid.splits), block(p.grid.threads);
+    const dim3 grid(p.row_blocks + (p.batch.batch - 1) / kCheckBatch + 1, p.grid.splits), block(p.grid.threads);
     if constexpr (sizeof(TI) == 2)
         if (vec == 8) {
             launch_pdl(kv_append_kernel<TI, TO, 8, INTER>, grid, block, 0, p);
@@ -251,6 +262,7 @@ int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id,
     p.err = device_error_word();
     if (!p.err) return fail(kBadHandle, "%s: no device error word", name);
     p.grid = rope_grid(rows, q_heads + 2 * c->kv_heads, p.shape.units);
+    p.row_blocks = (unsigned)((rows + (long long)p.grid.rows - 1) / p.grid.rows);
     auto launch = [&](auto in, auto out) {
         if (interleaved) launch_append<decltype(in), decltype(out), true>(p, vec);
         else launch_append<decltype(in), decltype(out), false>(p, vec);

@@ -36,6 +36,10 @@ struct KvBatch {
     int batch, rows, max_pages, prefix_len;
 };
 
+__device__ __forceinline__ bool kv_rows_fit(const KvBatch &batch, int first, int next) {
+    return 0 <= first && first <= next && next <= batch.rows;
+}
+
 // The sequences [first, last) that can own one of the rows row0 .. row0 + n - 1: all of a small batch; of a large one what
 // lies between two of 256 evenly spaced starts, so that a block looks at a few hundred sequences and not at all of them.
 // range: two ints of shared memory.  Ends with the block synchronised.
@@ -59,16 +63,16 @@ __device__ __forceinline__ int2 kv_range(int *range, const int *__restrict__ sta
     return make_int2(range[0], range[1]);
 }
 
-// The sequences of the block's rows row0 .. row0 + n - 1 into owner[] (shared memory; -1 behind the last sequence).
-// Every thread looks at some of the sequences, so there is no chain of dependent loads as in a search.  Ends with the
-// block synchronised.
-__device__ __forceinline__ void kv_owners(int *owner, int *range, const int *__restrict__ start, int batch, int row0, int n,
-                                          int tid, int threads) {
+// The sequences of the block's rows row0 .. row0 + n - 1 into owner[] (shared memory; -1 behind the last sequence, and for one
+// whose rows do not fit the call's).  Every thread looks at some of the sequences, so there is no chain of dependent loads
+// as in a search.  Ends with the block synchronised.
+__device__ __forceinline__ void kv_owners(int *owner, int *range, const KvBatch &batch, int row0, int n, int tid, int threads) {
     for (int i = tid; i < n; i += threads) owner[i] = -1;
-    const int2 some = kv_range(range, start, batch, row0, n, tid, threads);
+    const int2 some = kv_range(range, batch.start, batch.batch, row0, n, tid, threads);
     __syncthreads();
     for (int b = some.x + tid; b < some.y; b += threads) {
-        const int lo = max(start[b], row0), hi = min(start[b + 1], row0 + n);
+        const int first = batch.start[b], next = batch.start[b + 1];
+        const int lo = max(first, row0), hi = kv_rows_fit(batch, first, next) ? min(next, row0 + n) : lo;
         for (int t = lo; t < hi; ++t) owner[t - row0] = b;
     }
     __syncthreads();
