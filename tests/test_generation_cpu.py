@@ -61,3 +61,28 @@ def test_integers_of_other_types(lib):
     with pytest.raises(TypeError):
         native.call(lib.draft_verify_dev, *(args[:-1] + [100.0]))
     assert set(native.PLAIN_INTS) <= set(native.SIGNATURES)
+
+
+def test_arguments_of_the_plain_entry_points(lib):
+    """Direct calls and calls through the Python classes refuse what is no integer, and a wrong number of arguments."""
+    args = {"rope_dev": [1, 0, 512, 2, 0, 512, 3, 4, 1, 8, 4, 128, 64, 0, 0], "zilla_kv_append": [77] + [1] * 22,
+            "zilla_kv_attend": [77] + [1] * 13 + [C.c_float(1.0), 1], "draft_verify_dev": [1, 100, 2, 100, 3, 4, 5, 6, 7, 2, 6, 100]}
+    assert set(args) == native.PLAIN_INTS
+    for name, ok in args.items():
+        fn = getattr(lib, name)
+        assert fn(*ok) == -1, name
+        assert fn(*[np.int32(a) if isinstance(a, int) else a for a in ok]) == -1 and fn(*([True] + ok[1:])) == -1
+        for few in (ok[:-1], ok + [0], []):
+            with pytest.raises(TypeError):
+                fn(*few)
+        for at in (0, 3, len(ok) - 1):
+            for bad in (None, "2", b"2", 2.0, C.c_float(2.0), C.c_int(2), [2]):
+                with pytest.raises(TypeError):
+                    fn(*(ok[:at] + [bad] + ok[at + 1:]))
+                with pytest.raises(TypeError):
+                    native.call(fn, *(ok[:at] + [bad] + ok[at + 1:]))
+    for scale in (1, 0.5, np.float32(0.5), np.float64(0.5)):
+        assert lib.zilla_kv_attend(*(args["zilla_kv_attend"][:14] + [scale, 1])) == -1
+    for scale in (None, "1", b"1", C.c_int(1)):
+        with pytest.raises(TypeError):
+            lib.zilla_kv_attend(*(args["zilla_kv_attend"][:14] + [scale, 1]))

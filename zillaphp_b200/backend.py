@@ -195,14 +195,14 @@ class B200Backend:
 
     def ropeDev(self, xId, xOff, xLd, yId, yOff, yLd, posId, tableId, type, rows, heads, headDim, rotDim,  # noqa: A002,N802,N803,E501
                 interleaved=0, inverse=0):
-        rc = native.call(self.ffi.rope_dev, xId, xOff, xLd, yId, yOff, yLd, posId, tableId, type, rows, heads, headDim,
-                         rotDim, interleaved, inverse)
+        rc = self.ffi.rope_dev(xId, xOff, xLd, yId, yOff, yLd, posId, tableId, type, rows, heads, headDim, rotDim,
+                               interleaved, inverse)
         if rc:
             self._check(rc, "rope_dev")
 
     def draftVerifyDev(self, pId, pLd, qId, qLd, draftId, uId, startId, tokensId, acceptedId, batch, rows, vocab):  # noqa: N802,N803,E501
-        rc = native.call(self.ffi.draft_verify_dev, pId, pLd, qId, qLd, draftId, uId, startId, tokensId, acceptedId, batch,
-                         rows, vocab)
+        rc = self.ffi.draft_verify_dev(pId, pLd, qId, qLd, draftId, uId, startId, tokensId, acceptedId, batch, rows,
+                                       vocab)
         if rc:
             self._check(rc, "draft_verify_dev")
 

@@ -30,17 +30,17 @@ class PagedKv:
                q_heads: int, max_pages: int, prefix_len: int = 0, table_id: int = 0, rot_dim: int = 0,
                interleaved: int = 0) -> None:
         """Stores the new rows' K (rotated) and V in their pages and the rotated Q in qout (zilla_kv_append)."""
-        if native.call(self.lib.zilla_kv_append, self.id, x_type, q_id, q_off, q_ld, k_id, k_off, k_ld, v_id, v_off, v_ld,
-                       qout_id, start_id, len_id, pages_id, batch, rows, q_heads, max_pages, prefix_len, table_id, rot_dim,
-                       interleaved):
+        if self.lib.zilla_kv_append(self.id, x_type, q_id, q_off, q_ld, k_id, k_off, k_ld, v_id, v_off, v_ld, qout_id,
+                                    start_id, len_id, pages_id, batch, rows, q_heads, max_pages, prefix_len, table_id, rot_dim,
+                                    interleaved):
             raise ZillaError(f"zilla_kv_append failed. ({native.last_error()})")
 
     def attend(self, q_id: int, out_id: int, start_id: int, len_id: int, pages_id: int, prefix_pages_id: int, batch: int,
                rows: int, q_heads: int, max_pages: int, prefix_len: int, max_new: int, max_len: int, scale: float,
                work_id: int = 0) -> None:
         """Attention of the new rows over the prefix and their sequence's own keys (zilla_kv_attend)."""
-        if native.call(self.lib.zilla_kv_attend, self.id, q_id, out_id, start_id, len_id, pages_id, prefix_pages_id, batch,
-                       rows, q_heads, max_pages, prefix_len, max_new, max_len, c_float(scale), work_id):
+        if self.lib.zilla_kv_attend(self.id, q_id, out_id, start_id, len_id, pages_id, prefix_pages_id, batch, rows,
+                                    q_heads, max_pages, prefix_len, max_new, max_len, c_float(scale), work_id):
             raise ZillaError(f"zilla_kv_attend failed. ({native.last_error()})")
 
     def attend_work(self, batch: int, rows: int, q_heads: int, prefix_len: int, max_new: int, max_len: int) -> int:

@@ -118,10 +118,31 @@ SIGNATURES: dict[str, tuple] = {
     "zilla_dp_detach": (I, [I]),
 }
 
-# Entry points of many integers that are called once a token: their argtypes stay unset, as ctypes passes plain ints by
-# itself in a third of the time that converting them through argtypes takes (0.8 us against 2.5 us for 15 arguments);
-# `call` below is the way to them.
+# Entry points of many integers that are called once a token.  ctypes passes plain ints by itself in a third of the time that
+# converting them through argtypes takes, but then it also takes None, strings and any number of arguments.  So their
+# argtypes stay unset behind `_checked` (zilla_kv_append's 23 arguments: 0.85 us, 1.9 us through argtypes).
 PLAIN_INTS = {"rope_dev", "zilla_kv_append", "zilla_kv_attend", "draft_verify_dev"}
+
+
+def _checked(raw, argtypes):
+    """raw for arguments of its signature, ints and c_floats; integers and floats of other types (numpy's) are converted,
+    anything else and a wrong number of arguments raise TypeError."""
+    kinds = [int if t is I else t for t in argtypes]
+    count = len(kinds)
+
+    def convert(args):
+        if len(args) != count:
+            raise TypeError(f"{raw.__name__} takes {count} arguments, not {len(args)}.")
+        return raw(*[a if type(a) is k else operator.index(a) if k is int else k(a) for a, k in zip(args, kinds)])
+
+    def ints(*args):   # the sum is an int if all are; of None, a string and the like there is none
+        return raw(*args) if len(args) == count and type(sum(args)) is int else convert(args)
+
+    def mixed(*args):
+        return raw(*args) if [*map(type, args)] == kinds else convert(args)
+
+    return ints if kinds == [int] * count else mixed
+
 
 _lib: C.CDLL | None = None
 
@@ -139,18 +160,17 @@ def load() -> C.CDLL:
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = res
-        if name not in PLAIN_INTS:
+        if name in PLAIN_INTS:
+            setattr(lib, name, _checked(fn, args))
+        else:
             fn.argtypes = args
     _lib = lib
     return lib
 
 
 def call(fn, *args) -> int:
-    """Calls a function of PLAIN_INTS; integers of other types (numpy's) are converted, anything else is refused."""
-    try:
-        return fn(*args)
-    except C.ArgumentError:
-        return fn(*[a if isinstance(a, C.c_float) else operator.index(a) for a in args])
+    """fn(*args), with the checks of fn."""
+    return fn(*args)
 
 
 def last_error() -> str:
