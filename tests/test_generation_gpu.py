@@ -966,3 +966,36 @@ def test_append_rows_that_do_not_fit_are_recorded(bufs, start, bad, spare):
         want, want_k = torch.where(got == 7.0, got, want), torch.where(got_k == 3.0, got_k, want_k)
     assert torch.equal(got, want) and torch.equal(got_k, want_k) and torch.equal(got_v, want_k)
     kv.close()
+
+
+@pytest.mark.parametrize("dtype,dim,hq,hk,page,prefix,new,length", [
+    ("bf16", 128, 8, 2, 64, 0, [300, 1, 513], [300, 40, 700]),          # prompts from their first token, and behind earlier ones
+    ("fp16", 64, 16, 2, 16, 100, [257, 64, 0, 130], [257, 64, 9, 1000]),
+    ("bf16", 128, 8, 1, 64, 1500, [400, 129], [400, 500]),              # the prefix on tcgen05
+    ("fp16", 32, 4, 4, 128, 2500, [1, 650], [300, 651]),
+    ("bf16", 64, 2, 2, 32, 3, [190] * 3, [190, 1, 200]),                # more new rows than keys
+])
+def test_attend_prompts(bufs, dtype, dim, hq, hk, page, prefix, new, length):
+    """Hundreds of new rows a sequence, as a prompt's pass has them."""
+    run_attend(bufs, dtype, new, length, hq, hk, dim, page, prefix, 2)
+
+
+@pytest.mark.parametrize("dtype,hq,dim,rot,interleaved", [("bf16", 6, 64, 64, 0), ("fp16", 3, 128, 40, 1), ("bf16", 5, 32, 30, 0)])
+def test_append_in_place(bufs, dtype, hq, dim, rot, interleaved):
+    """The queries rotated where they lie, for rows of the cache's type without gaps."""
+    T, new = R.DT[dtype], [40, 0, 3]
+    start, pages, _, count, most = batch_of(new, [50, 7, 3], 0, 16, 81)
+    g = torch.Generator().manual_seed(82)
+    rows = start[-1] + 2
+    q, k, v = (torch.randn((rows, h, dim), generator=g).to(T) for h in (hq, 1, 1))
+    kv = PagedKv(count, 16, 1, dim, dtype)
+    table = bufs.new(rot + 2)
+    bufs.be.ropeTableDev(table, rot)
+    iq = bufs.put(q)
+    kv.append(R.CODE[dtype], iq, 0, hq * dim, bufs.put(k), 0, dim, bufs.put(v), 0, dim, iq, bufs.put(i32(start)), bufs.put(i32([50, 7, 3])), bufs.put(pages),
+              3, rows, hq, most, 11, table, rot, interleaved)
+    got, pos = bufs.get(iq, q.shape, T), 11 + torch.tensor(list(range(10, 50)) + [0, 1, 2])
+    ref, size = R.rotate(q[:-2], pos, rot, interleaved, R.rates(rot))
+    assert ((got[:-2].double() - ref).abs() <= size * (R.ROTATION + R.far(pos)) + R.half_step(ref, T)).all()
+    assert torch.equal(got[-2:], q[-2:])
+    kv.close()
