@@ -999,3 +999,24 @@ def test_append_in_place(bufs, dtype, hq, dim, rot, interleaved):
     assert ((got[:-2].double() - ref).abs() <= size * (R.ROTATION + R.far(pos)) + R.half_step(ref, T)).all()
     assert torch.equal(got[-2:], q[-2:])
     kv.close()
+
+
+def test_a_buffer_that_took_the_place_of_a_caches(bufs):
+    """A cache whose buffer was freed stays refused when a new buffer has the handle and the memory of the old one, and does not
+    free that one."""
+    be, lib = bufs.be, native.load()
+    for which in range(2):
+        kv = PagedKv(4, 16, 2, 32, "bf16")
+        freed = (kv.k_id, kv.v_id)[which]
+        be.bufferFree(freed)
+        mine = [be.bufferAlloc(4 * 16 * 2 * 32 // 2) for _ in range(3)]
+        assert freed in mine                                    # the first free handle, and as a rule the same memory
+        want = torch.arange(4 * 16 * 2 * 32 // 2).float()
+        for i in mine:
+            bufs.write(i, want)
+        assert lib.zilla_kv_k_id(kv.id) == -1 and lib.zilla_kv_v_id(kv.id) == -1
+        assert lib.zilla_kv_attend_work(kv.id, 1, 1, 2, 0, 1, 16) == -1
+        kv.close()
+        for i in mine:
+            assert torch.equal(bufs.get(i, want.shape, torch.float32), want)
+            be.bufferFree(i)

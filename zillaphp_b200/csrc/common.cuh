@@ -32,6 +32,9 @@ void count_launch(unsigned n = 1);
 float *ptr(int id);
 // Capacity in floats of a registry handle (0 if invalid).
 size_t capacity(int id);
+// The number of the allocation behind a registry handle (0 if invalid): another
+// one once the handle has been freed, also where handle and memory are the same.
+unsigned long long allocation(int id);
 
 // One buffer argument of an entry point: its handle, the floats that the call
 // reads or writes in it, and its name in the error text.

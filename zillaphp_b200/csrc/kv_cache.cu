@@ -114,7 +114,7 @@ const KvCache *kv_get(int id) {
     auto it = g_caches.find(id);
     if (it == g_caches.end()) return nullptr;
     const KvCache *c = it->second;
-    return ptr(c->k_id) == c->k && ptr(c->v_id) == c->v ? c : nullptr;
+    return allocation(c->k_id) == c->k_made && allocation(c->v_id) == c->v_made ? c : nullptr;
 }
 
 }  // namespace zb
@@ -149,6 +149,8 @@ int zilla_kv_create(int pages, int page, int kv_heads, int head_dim, int type) {
     if (!rc) {
         c->k = ptr(c->k_id);
         c->v = ptr(c->v_id);
+        c->k_made = allocation(c->k_id);
+        c->v_made = allocation(c->v_id);
         cudaMemsetAsync(c->k, 0, floats * sizeof(float), stream());
         cudaMemsetAsync(c->v, 0, floats * sizeof(float), stream());
         cudaStreamSynchronize(stream());   // zero before work on any other stream
@@ -178,8 +180,8 @@ int zilla_kv_destroy(int kv) {
     auto it = g_caches.find(kv);
     if (it == g_caches.end()) return fail(kBadHandle, "zilla_kv_destroy: unknown cache %d", kv);
     KvCache *c = it->second;
-    if (ptr(c->k_id) == c->k) zilla_buffer_free(c->k_id);
-    if (ptr(c->v_id) == c->v) zilla_buffer_free(c->v_id);
+    if (allocation(c->k_id) == c->k_made) zilla_buffer_free(c->k_id);
+    if (allocation(c->v_id) == c->v_made) zilla_buffer_free(c->v_id);
     g_caches.erase(it);
     delete c;
     return kOk;

@@ -13,6 +13,7 @@ namespace zb {
 struct KvCache {
     int pages = 0, page = 0, page_log2 = 0, kv_heads = 0, head_dim = 0, type = kBf16;
     int k_id = 0, v_id = 0;
+    unsigned long long k_made = 0, v_made = 0;   // their allocations: a freed buffer's handle may come back as another's
     void *k = nullptr, *v = nullptr;
     CUtensorMap k_map, v_map;   // [pages * kv_heads * page][head_dim], box {min(head_dim, 64), box_rows}
     int box_rows = 0;           // rows of one TMA box: a page, 64 at most

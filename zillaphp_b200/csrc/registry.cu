@@ -19,6 +19,7 @@ struct Slot {
     size_t n;
     int used;
     int device;   // the device the memory is on
+    unsigned long long serial;   // the allocation's number
 };
 Slot g_slots[kSlots];
 cudaStream_t g_own_stream = nullptr;
@@ -28,6 +29,7 @@ unsigned long long g_launches = 0;
 int g_last_status = 0;
 char g_last_error[512] = "";
 int g_sms = 0;
+unsigned long long g_allocations = 0;
 }  // namespace
 
 namespace {
@@ -86,6 +88,8 @@ size_t capacity(int id) {
     if (id <= 0 || id >= kSlots || !g_slots[id].used) return 0;
     return g_slots[id].n;
 }
+
+unsigned long long allocation(int id) { return ptr(id) ? g_slots[id].serial : 0; }
 
 int check_buffers(const char *name, std::initializer_list<BufferNeed> needs) {
     for (const BufferNeed &b : needs) {
@@ -147,7 +151,7 @@ int zilla_buffer_alloc(unsigned long n_floats) {
         }
         int dev = 0;
         cudaGetDevice(&dev);
-        g_slots[i] = {p, (size_t)n_floats, 1, dev};
+        g_slots[i] = {p, (size_t)n_floats, 1, dev, ++g_allocations};
         device_error_word();   // exists before any op on a buffer runs, so an op's first call may be captured
         return i;
     }
@@ -158,7 +162,7 @@ void zilla_buffer_free(int id) {
     if (id <= 0 || id >= kSlots || !g_slots[id].used) return;
     cudaStreamSynchronize(stream());
     cudaFree(g_slots[id].p);
-    g_slots[id] = {nullptr, 0, 0, 0};
+    g_slots[id] = {nullptr, 0, 0, 0, 0};
 }
 
 int zilla_buffer_upload(int id, const float *host, unsigned long n_floats) {
