@@ -427,7 +427,8 @@ long zilla_kv_attend_work(int kv, int batch, int rows, int q_heads, int prefix_l
  * from max(p_a - q_a, 0) (from p_a where that is zero throughout), else from p_k:
  * the lowest t whose sum of weights up to t is above u_k times the whole sum.
  * tokens [rows]: the accepted drafts, the drawn token, then -1; accepted[b] = a.
- * Sums are good to 2^-42 of themselves (2^-39 at the largest vocab, 2^28).
+ * Weights are summed in 64 bits (to 2^-47 of the sum up to a vocab of 131,072,
+ * 2^-37 at the largest, 2^28).
  * q_id 0: drafts made with certainty (q is one at the draft).  NaN and negative
  * weights count as zero, infinite p and q as the largest finite number; u_k >= 1
  * takes the last token with a weight; no weight at all gives token 0.  A draft

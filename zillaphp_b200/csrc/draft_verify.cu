@@ -7,8 +7,9 @@
 //   w = max(p_a - q_a, 0) where a draft failed, p_a behind the last one;
 //   the token drawn is the lowest t with w_0 + ... + w_t > r (w_0 + ... + w_{V-1}), r = u_k.
 // fp32 sums over a large vocabulary are off by more than the distance between neighbouring borders, and would make
-// the token depend on how a row is split: differences are exact and sums are kept to 42 bits, eight weights as a pair of
-// fp32 numbers, everything else in fp64 (whose own roundings count from some 2^24 entries on: 39 bits at 2^28).
+// the token depend on how a row is split: weights are differences in fp64 and summed in fp64, a thread's four together, so
+// that its chain of additions is short (192 rows of 100,003 in a graph of calls 28.6 us; one after the other 29.9).  A sum
+// is off by at most 2^-53 of itself for each addition behind each other: V / 4096 a thread and some 50 to join them.
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -41,42 +42,12 @@ __device__ __forceinline__ double residual(float p, float q) {
     return p > q ? (double)fminf(p, FLT_MAX) - (double)fmaxf(q, -FLT_MAX) : 0.0;
 }
 
-// The sum of up to kPairTerms residuals as an unevaluated sum hi + lo of fp32 numbers: the difference p - q = d + e is exact
-// (Dekker 1971, p > q >= 0; a negative q costs at most lo's rounding), hi + d = h + t too (Knuth's two-sum), and lo
-// takes e and t.  Eleven additions on the fp32 pipe; the same sum in fp64 is bound by two conversions an element (47 us
-// against 29 us for 192 rows of 100,003).
-// lo is a plain fp32 sum: behind n terms of sum S it is at most (n + 1) 2^-24 S, and each step rounds it and e + t, so that
-// hi + lo is off by (n^2 / 2 + 2 n + 1) 2^-48 S at most: 2^-42 S for the eight terms that go into an fp64 sum together.
-// (A pair over a lane's whole part of a row has no such bound: 34 bits were left of 2000 terms behind one of 0.75.)
-constexpr int kPairTerms = 8;
-struct PairSum {
-    float hi = 0.0f, lo = 0.0f;
-    __device__ __forceinline__ void add(float p, float q, bool keep) {
-        if (!(p > q) || !keep) p = q = 0.0f;
-        p = fminf(p, FLT_MAX);
-        const float d = p - q, e = (p - d) - q;
-        const float h = hi + d, b = h - hi, t = (hi - (h - b)) + (d - b);
-        hi = h;
-        lo += e + t;
-    }
-};
-
-// A warp's sum in fp64 throughout, for weights near the end of fp32's range.  Not inlined: its registers stay out of the kernel.
-__device__ __noinline__ double wide_sum(const float *p, const float *q, int skip, int begin, int end, int lane) {
-    double s = 0.0;
-    for (int i = begin + lane; i < end; i += 32)
-        if (i != skip) s += residual(p[i], q ? q[i] : 0.0f);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-}
-
 // Bound by HBM: one row of p, and one of q where a draft failed, read once by the sequence's cluster.
 // Each warp sums one segment of the row; the segments' sums meet in the cluster's shared memory, and the
 // block that owns the crossing segment reads it again (it is in L2) to find the token.
 // Six blocks an SM (40 registers a thread), so that blocks that look for their row or for their token leave enough others
-// that stream: 29 us against 36 with four.  ALONE: so few blocks that no SM has a second one; then a thread's own loads
-// have to cover the latency, and four times as many are in flight (one row of 131,072: 7.9 against 7.2 us).
+// that stream: 28.6 us against 31.2 with four.  ALONE: so few blocks that no SM has a second one; then a thread's own loads
+// have to cover the latency, and four times as many are in flight (one row of 131,072: 7.2 against 8.5 us).
 template <bool VEC, bool ALONE>
 __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_kernel(const VerifyParams a) {
     __shared__ double sums[kVerifyWarps];                      // read by the whole cluster
@@ -136,22 +107,14 @@ __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_ke
         const long long lo = (long long)(rank * kVerifyWarps + warp) * a.seg;
         const int begin = (int)min(lo, (long long)V), end = (int)min(lo + a.seg, (long long)V);
         double s = 0.0;
-        PairSum sum;
-        auto take = [&](int i, float x, float y) { sum.add(x, y, i != skip); };
-        auto flush = [&] {
-            s += (double)sum.hi + (double)sum.lo;
-            sum = PairSum();
-        };
+        auto weigh = [&](int i, float x, float y) { return i == skip ? 0.0 : residual(x, y); };
         // a batch of loads in front of its sums: 64 bytes a thread in flight, or 256
         auto stream = [&](auto with_q) {
             constexpr bool kQ = decltype(with_q)::value;
             if constexpr (VEC) {
                 constexpr int kBatch = (kQ ? 2 : 4) * (ALONE ? 4 : 1);
-                auto part4 = [&](int i, const float4 &x, const float4 &y) {
-                    take(i, x.x, y.x);
-                    take(i + 1, x.y, y.y);
-                    take(i + 2, x.z, y.z);
-                    take(i + 3, x.w, y.w);
+                auto take4 = [&](int i, const float4 &x, const float4 &y) {
+                    s += (weigh(i, x.x, y.x) + weigh(i + 1, x.y, y.y)) + (weigh(i + 2, x.z, y.z) + weigh(i + 3, x.w, y.w));
                 };
                 int i = begin + 4 * lane;
                 const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -163,16 +126,11 @@ __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_ke
                         y[e] = kQ ? *reinterpret_cast<const float4 *>(q + i + 128 * e) : zero;
                     }
 #pragma unroll
-                    for (int e = 0; e < kBatch; ++e) {
-                        part4(i + 128 * e, x[e], y[e]);
-                        if ((e + 1) % (kPairTerms / 4) == 0) flush();
-                    }
+                    for (int e = 0; e < kBatch; ++e) take4(i + 128 * e, x[e], y[e]);
                 }
-                for (; i + 3 < end; i += 128) {
-                    part4(i, *reinterpret_cast<const float4 *>(p + i), kQ ? *reinterpret_cast<const float4 *>(q + i) : zero);
-                    flush();
-                }
-                for (; i < end; ++i) take(i, p[i], kQ ? q[i] : 0.0f);   // the row's last one to three elements, one lane's
+                for (; i + 3 < end; i += 128)
+                    take4(i, *reinterpret_cast<const float4 *>(p + i), kQ ? *reinterpret_cast<const float4 *>(q + i) : zero);
+                for (; i < end; ++i) s += weigh(i, p[i], kQ ? q[i] : 0.0f);   // the row's last one to three elements, one lane's
             } else {
                 constexpr int kBatch = (kQ ? 4 : 8) * (ALONE ? 4 : 1);
                 int i = begin + lane;
@@ -184,23 +142,15 @@ __global__ void __launch_bounds__(kVerifyThreads, ALONE ? 1 : 6) draft_verify_ke
                         y[e] = kQ ? q[i + 32 * e] : 0.0f;
                     }
 #pragma unroll
-                    for (int e = 0; e < kBatch; ++e) {
-                        take(i + 32 * e, x[e], y[e]);
-                        if ((e + 1) % kPairTerms == 0 || e == kBatch - 1) flush();
-                    }
+                    for (int e = 0; e < kBatch; e += 2) s += weigh(i + 32 * e, x[e], y[e]) + weigh(i + 32 * (e + 1), x[e + 1], y[e + 1]);
                 }
-                for (int n = 1; i < end; i += 32, ++n) {
-                    take(i, p[i], kQ ? q[i] : 0.0f);
-                    if (n % kPairTerms == 0) flush();
-                }
+                for (; i < end; i += 32) s += weigh(i, p[i], kQ ? q[i] : 0.0f);
             }
-            flush();
         };
         if (q) stream(std::true_type());
         else stream(std::false_type());
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (!(s < INFINITY)) s = wide_sum(p, q, skip, begin, end, lane);   // a pair has passed fp32's range
         if (lane == 0) sums[warp] = s;
         cluster.sync();
         for (int i = tid; i < kVerifyMaxCluster * kVerifyWarps; i += kVerifyThreads)
@@ -322,9 +272,9 @@ int clusters_at_once(void (*kernel)(VerifyParams), bool vec, int ranks) {
 }
 
 // Blocks to a sequence: the most with which all sequences run at once, and in a second round, a third, ... only where a block
-// would have more than 24576 elements otherwise (its start and its search at the end then count for little).  One round
-// against eight blocks to a sequence: 192 rows of 32,000 14.2 us (four blocks) against 16.4, 384 rows 24.5 (two) against
-// 31.4; 192 rows of 100,003 30.5 (four) against 29.6.  A block has 512 elements at least.
+// would have more than 24576 elements otherwise (its start and its search at the end then count for little).  Measured against
+// eight blocks to a sequence: 192 rows of 32,000 11.4 us against 13.8, 384 rows 21.0 (two blocks) against 27.1; 192 rows of
+// 100,003 take eight, 28.6 against 29.6 with four.  A block has 512 elements at least.
 int choose_ranks(void (*kernel)(VerifyParams), bool vec, int batch, int vocab) {
     const int most = std::max(1, std::min(kVerifyMaxCluster, vocab / 512)), least = std::min(most, (vocab + 24575) / 24576);
     const int fit = clusters_at_once(kernel, vec, least);
