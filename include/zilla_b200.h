@@ -411,6 +411,8 @@ int zilla_kv_append(int kv, int x_type, int q_id, int q_off, int q_ld, int k_id,
  * is recorded and its rows are left as they are).  Whatever lies in pages behind
  * a sequence's length does not matter; V of the tokens within it has to be
  * finite.  A page number outside the cache counts as keys and values of zero.
+ * Scores, sums and partial results are fp32; the softmax weights are rounded to
+ * the cache's type before they meet V, and the result once more at the end.
  * work: zilla_kv_attend_work floats (0: work_id is not looked at) that no other
  * call in flight uses. */
 int zilla_kv_attend(int kv, int q_id, int out_id, int start_id, int len_id, int pages_id, int prefix_pages_id, int batch,

@@ -618,11 +618,13 @@ constexpr int kTcRows = 16, kTcWork = 12288;
 //   t = units / n * tile + start,  plus what the other SMs - n have not moved by then at the whole machine's rate,
 // and the n that minimises it is taken, among the multiples of the row tiles where they are few.  A tile of 256 rows and 128
 // keys takes 2.2 us with head_dim 128 in a loop of such calls, which runs into the power limit (1.7 at full clock: 88% of the
-// measured matrix rate), 1.8 with 64; 12 us stands for the start, the queries and the parts; an SM draws about 45 GB/s, all
-// together 5.6 TB/s.  Lengths are on the device: half of their bound is assumed.  128 sequences of up to 2048 keys behind
-// 16384 (n = 96) take 199 us at full clock, with 80 blocks 222, with 112 204; 32 sequences of up to 700 behind 2029 (n = 64)
-// 24.6, with 32 blocks 21.1, with 96 25.5 (the other kernel's own start, which this leaves out; with it that shape gains 3%
-// and 64 sequences behind 1000 keys lose 7%).
+// measured matrix rate), 1.8 with 64; 12 us stands for the start, the queries and the parts (a fit, not measured apart); an SM draws about 45 GB/s, all
+// together 5.6 TB/s.  Lengths are on the device: half of their bound is assumed.
+// Where the rule lands, in graphs of calls: 128 sequences of up to 2048 keys behind 16384 take 96 blocks, 209 to 231 us with the
+// clock under the power limit (80 blocks 238, 112 230, 148 237); 64 drafts of head_dim 64 behind 4001 take 133, 35.6 us (96
+// blocks 35.0, 64 40.8); 64 sequences behind 1000 take 44, 28.8 to 32.6 us (32 blocks 29.2, 64 30.1, 148 33.7); 32 sequences of
+// up to 700 behind 2029 take 85, 24.4 us, where 32 would take 20.3 and 64 23.4: every count from 64 to 85 has the same longest
+// block, and of equals the largest is taken.
 int choose_tc_blocks(const KvCache &c, int row_tiles, long long units, double own_bytes) {
     const int sms = sm_count();
     const double tile = c.head_dim == 128 ? 2.2e-6 : 1.8e-6, start = 12e-6, one = 45e9, all = 5.6e12;

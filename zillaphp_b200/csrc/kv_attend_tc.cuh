@@ -14,7 +14,9 @@
 // never waits for an MMA of its own stream.  One buffer of 128 keys makes softmax, P V and Q K^T a chain: 206 us against 199
 // at full clock for the large batch above, with each row's softmax shared by two warps and the streams issued in turn (260 if
 // both streams' MMAs are issued side by side, which keeps them in step).  That sharing alone changes nothing (200), nor does
-// a delay between the streams: a tile takes 1.7 us with head_dim 128, 88% of what the measured matrix rate would give.
+// a delay between the streams.  A further tile takes 1.7 us with head_dim 128 at full clock (from 16384 to 32768 shared keys),
+// 88% of what the measured matrix rate would give; the whole kernel of the large batch, with its start, its parts, 1804 rows in
+// 2048 and 96 blocks, has the tensor pipe active for 48% of their SMs' time.
 // ref is the row's maximum as of its last change: it follows the true maximum only when that has passed it
 // by 2^8 (then O and l are rescaled), so that O rarely has to travel through registers; weights stay
 // below 2^8 and l and O carry the same factor, so the quotient does not change.  Before the first finite score (a key may
